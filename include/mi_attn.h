@@ -335,6 +335,102 @@ mi_status mi_matvec_q4(const mi_f16* x, const uint32_t* w_packed,
                        int32_t group_size, float* out, int32_t out_dim,
                        int32_t in_dim, mi_stream stream);
 
+/* --------------------------------------- rotary positions, paged cache -- */
+
+/* Types of the strided inputs below. */
+typedef enum mi_dtype { MI_F32 = 0, MI_F16 = 1, MI_BF16 = 2 } mi_dtype;
+
+/* Rotary positions of x [n][heads][head_dim] (head_dim 256), with an optional
+ * RMS norm before: y = x / sqrt(mean x^2 + eps) * norm_w (bf16 [D]; NULL: no
+ * norm), then the pairs (a, b) of the first rotary_dim columns become
+ *   factor * (a cos t - b sin t, b cos t + a sin t), t = position * frequency.
+ * Pairs are columns (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with
+ * `interleaved`; the other columns pass.  host_freq: rotary_dim / 2 frequencies
+ * (host memory, copied by the call), scaled by the caller for a long context;
+ * angles are formed in 64 bits.  positions: int32 [n], or int64 with
+ * positions_64.  x_type, out_type: any mi_dtype; strides in elements, the 256
+ * columns contiguous, every row 16-byte aligned; out is contiguous and may be x
+ * itself (same type and strides), else must not overlap it.  rotary_dim: a
+ * multiple of 8, at most 256.  Async.  Beside q_head_norm_rope / k_head_norm_rope
+ * (src/math_util.rs:501-593), which know one layout and no scaling. */
+mi_status mi_rope_apply(const void* x, int32_t x_type, int64_t token_stride, int64_t head_stride,
+                        int32_t n, int32_t heads, int32_t head_dim, const void* positions,
+                        int32_t positions_64, const uint16_t* norm_w, float eps,
+                        const double* host_freq, int32_t rotary_dim, int32_t interleaved,
+                        double factor, void* out, int32_t out_type, mi_stream stream);
+
+/* The paged 4-bit KV cache of a batch of sequences (one layer).
+ *   pages: [num_pages][G][page_rows / 32][MI_PAGED_TILE_BYTES], 16-byte aligned;
+ *     page_rows a power of two, 32 to 1024.  A tile is 32 rows of one KV head:
+ *     4-bit codes of K (4096 bytes) and V (4096), then scales and offsets in f16
+ *     per row and group of 64 columns, of K (512) and V (512).  A value is
+ *     f16((16 + code) * scale + offset).  csrc/paged.h has the order within a tile.
+ *   block_table: int32 [batch][table_cols], the page of rows
+ *     [j page_rows, (j + 1) page_rows) of a sequence; unused entries -1.
+ *   kv_len: int32 [batch], rows of each sequence, those of this call included.
+ *   cu_q: int32 [batch + 1], ascending from 0: tokens cu_q[s] .. cu_q[s + 1] - 1
+ *     of the call belong to sequence s and are its last rows (the last token is
+ *     row kv_len[s] - 1).  NULL: one token per sequence.  Tokens from
+ *     cu_q[batch] on belong to none: their outputs are left as they were.
+ * The tables are device memory and are read by the kernels, so a captured call
+ * follows their contents.  The kernels bound every access by them: a row whose
+ * page is not in the table (or whose entry is not a page of the pool) is not
+ * written, and reads as NaN; a token whose row would be negative (kv_len[s] less
+ * than its tokens: an empty sequence of a padded batch) is not written, reads as
+ * zero and attends nothing.  Two sequences of a call may share pages that it
+ * reads, not pages that it writes.  batch <= 65535.  G: any; q heads per KV head
+ * 1 to 16. */
+#define MI_PAGED_TILE_BYTES 9216
+
+/* Appends n tokens' K and V: K RMS-normed (k_norm_w, bf16 [D] or NULL), rotated
+ * at its row (as mi_rope_apply) and quantised, V quantised.  Scale and offset of
+ * a group: f16((max - min) / 15), f16(min - 16 scale); code: the nearest, ties to
+ * even; 64-bit arithmetic throughout.  A group that holds a NaN or an infinity,
+ * or whose scale or offset does not fit f16, is stored as NaN.  With q: q_out
+ * [n][H][D] f16 = q normed (q_norm_w) and rotated, in the same launch; q_out may
+ * be q (contiguous f16).  q, k, v: one mi_dtype, strides as for mi_rope_apply.
+ * Rows outside the call's keep their contents.  Beside kv_cache_append
+ * (src/math_util.rs:387-392). */
+mi_status mi_paged_append(void* pages, int64_t num_pages, int32_t page_rows,
+                          const int32_t* block_table, int32_t table_cols, const int32_t* kv_len,
+                          const int32_t* cu_q, int32_t batch, int32_t n, int32_t num_q_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t type, const void* q,
+                          int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                          int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                          int64_t v_token_stride, int64_t v_head_stride, const uint16_t* q_norm_w,
+                          const uint16_t* k_norm_w, float eps, const double* host_freq,
+                          int32_t rotary_dim, int32_t interleaved, double factor, mi_f16* q_out,
+                          mi_stream stream);
+
+/* The last rows of each sequence as f16: k_out, v_out [n][G][D], token cu_q[s] + i
+ * the row kv_len[s] - (cu_q[s + 1] - cu_q[s]) + i.  The counterpart of
+ * mi_kv_download for pages (to save, move or inspect rows). */
+mi_status mi_paged_read(const void* pages, int64_t num_pages, int32_t page_rows,
+                        const int32_t* block_table, int32_t table_cols, const int32_t* kv_len,
+                        const int32_t* cu_q, int32_t batch, int32_t n, int32_t num_kv_heads,
+                        int32_t head_dim, mi_f16* k_out, mi_f16* v_out, mi_stream stream);
+
+/* Attention of the call's tokens over the pages: token i of sequence s attends
+ * the rows up to its own, softmax(q . K^T / sqrt(D)) V, then out *= sigmoid(gate)
+ * when gate != NULL (f16 or f32: gate_type).  cu_q == NULL is a decode step (one
+ * token per sequence); prompts, chunks behind cached rows and drafts to verify go
+ * through cu_q.  max_q, max_len: at least every sequence's tokens and rows (a
+ * sequence beyond them gets NaN).  q: f16 [n][H][D], q and gate strided as for
+ * mi_rope_apply, out contiguous; out may be q's or gate's buffer (contiguous f16),
+ * else must not overlap them.  workspace: device memory, 16-byte aligned, of
+ * mi_attn_paged_workspace_size bytes for these sizes or larger ones; calls that
+ * may run at the same time need one each. */
+size_t mi_attn_paged_workspace_size(int32_t batch, int32_t n, int32_t max_q, int32_t max_len,
+                                    int32_t num_q_heads, int32_t num_kv_heads);
+mi_status mi_attn_paged(const void* pages, int64_t num_pages, int32_t page_rows,
+                        const int32_t* block_table, int32_t table_cols, const int32_t* kv_len,
+                        const int32_t* cu_q, int32_t batch, int32_t n, int32_t max_q,
+                        int32_t max_len, int32_t num_q_heads, int32_t num_kv_heads,
+                        int32_t head_dim, const mi_f16* q, int64_t q_token_stride,
+                        int64_t q_head_stride, const void* gate, int32_t gate_type,
+                        int64_t gate_token_stride, int64_t gate_head_stride, mi_f16* out,
+                        void* workspace, size_t workspace_bytes, mi_stream stream);
+
 /* ------------------------------------------------------------- profiling -- */
 
 /* Kernel timing with HIP events stamped by each dispatch on its launch
@@ -342,7 +438,8 @@ mi_status mi_matvec_q4(const mi_f16* x, const uint32_t* w_packed,
  * kernel granularity).  mi_prof_enable synchronises the device and clears
  * earlier records.  Kernel names: "attn_split", "attn_combine",
  * "attn_direct", "attn_prefill", "verify_wide", "kv_pack",
- * "qk_norm_rope", "matvec_bf16", "matvec_q4", "ragged_plan".
+ * "qk_norm_rope", "matvec_bf16", "matvec_q4", "ragged_plan", "rope_apply",
+ * "paged_append", "paged_read", "paged_attn", "paged_merge".
  * mi_prof_read returns the mean duration in microseconds and the number of
  * launches recorded since the last enable. */
 void mi_prof_enable(int on);

@@ -63,6 +63,15 @@ SIGNATURES = [
     ("mi_attn_step_proj", ST, [P, I32, P, P, P, P, P, I32, C.c_float, C.c_float, P, I64, P]),
     ("mi_matvec_bf16", ST, [P, P, P, I32, I32, P]),
     ("mi_matvec_q4", ST, [P, P, P, P, I32, P, I32, I32, P]),
+    ("mi_rope_apply", ST, [P, I32, I64, I64, I32, I32, I32, P, I32, P, C.c_float, P, I32, I32,
+                           C.c_double, P, I32, P]),
+    ("mi_paged_append", ST, [P, I64, I32, P, I32, P, P, I32, I32, I32, I32, I32, I32, P, I64, I64,
+                             P, I64, I64, P, I64, I64, P, P, C.c_float, P, I32, I32, C.c_double, P,
+                             P]),
+    ("mi_paged_read", ST, [P, I64, I32, P, I32, P, P, I32, I32, I32, I32, P, P, P]),
+    ("mi_attn_paged_workspace_size", SZ, [I32, I32, I32, I32, I32, I32]),
+    ("mi_attn_paged", ST, [P, I64, I32, P, I32, P, P, I32, I32, I32, I32, I32, I32, I32, P, I64,
+                           I64, P, I32, I64, I64, P, P, SZ, P]),
     ("mi_prof_enable", None, [C.c_int]),
     ("mi_prof_read", ST, [C.c_char_p, C.POINTER(C.c_double), C.POINTER(I64)]),
     ("mi_bench_mfma_ceiling", ST, [P, I32, I32, P, P, P]),

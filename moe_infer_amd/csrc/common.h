@@ -49,6 +49,17 @@ mi_status check_rope(const mi_kv* kv, int32_t rotary_dim, float rope_theta, floa
 // writes it (src/math_util.rs:524).
 void rope_inv_freq(float rope_theta, int32_t rotary_dim, float* inv_freq);
 
+// Strided rows [n][heads][kHeadDim] of an mi_dtype (strides in elements): a
+// known type, not null, 16-byte aligned, heads and tokens in order (rotary.hip).
+mi_status check_rows(const char* name, const void* p, int32_t type, int64_t token_stride,
+                     int64_t head_stride, int64_t heads);
+// Elements from the first to the last of such rows.
+inline int64_t rows_extent(int64_t n, int64_t heads, int64_t token_stride, int64_t head_stride) {
+  return (n - 1) * token_stride + (heads - 1) * head_stride + kHeadDim;
+}
+// Whether two byte ranges have a byte in common.
+bool overlaps(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes);
+
 // Workgroup barrier for LDS hand-offs only: waits for this wave's LDS
 // operations, not for its outstanding global loads (which __syncthreads
 // would drain), then synchronises the workgroup.

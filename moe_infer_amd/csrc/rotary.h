@@ -1,0 +1,175 @@
+// Rotary positions: y = (a cos t - b sin t, b cos t + a sin t) * factor for
+// the pairs (a, b) of the first rotary_dim columns, t = position * frequency.
+// Pairs are columns (i, i + rotary_dim / 2) ("half") or (2 i, 2 i + 1)
+// ("interleaved").  The frequencies come from the caller in 64 bits, already
+// scaled for a long context.
+//
+// Angles are formed and reduced in 64 bits: at position 10^6 an f32 product is
+// off by 0.06 rad.  After the reduction to [-pi/4, pi/4] sine and cosine are
+// their Taylor sums, in f32 to the terms r^9 and r^10 (the next are 2e-9) or in
+// f64 to r^15 and r^16 (5e-17).
+//
+// A wave holds one head of 256 columns, lane l the columns 4 l .. 4 l + 3; an
+// angle is computed once, in one lane, and fetched from it.
+#pragma once
+
+#include "common.h"
+
+namespace mi {
+
+struct RotaryPlan {
+  double freq[MI_ROPE_MAX_DIM / 2];
+  double factor;
+  int32_t half;         // rotary_dim / 2
+  int32_t interleaved;
+};
+
+// Checks and copies the caller's plan (host_freq may be null when rotary_dim
+// is 0).
+mi_status rotary_plan(const double* host_freq, int32_t rotary_dim, int32_t interleaved,
+                      double factor, RotaryPlan* out);
+
+// sin and cos of t (64 bits), as T.
+template <typename T>
+__device__ __forceinline__ void turn(double t, T& s, T& c) {
+  constexpr double kHi = 1.5707963267948966, kLo = 6.123233995736766e-17;  // pi / 2
+  const double k = rint(t * 0.63661977236758134308);
+  const T r = (T)fma(-k, kLo, fma(-k, kHi, t));
+  const T r2 = r * r;
+  T ps, pc;
+  if constexpr (sizeof(T) == 8) {
+    ps = fma(r2, -1.0 / 1307674368000.0, 1.0 / 6227020800.0);
+    ps = fma(r2, ps, -1.0 / 39916800.0);
+    ps = fma(r2, ps, 1.0 / 362880.0);
+    ps = fma(r2, ps, -1.0 / 5040.0);
+    ps = fma(r2, ps, 1.0 / 120.0);
+    ps = fma(r2, ps, -1.0 / 6.0);
+    pc = fma(r2, 1.0 / 20922789888000.0, -1.0 / 87178291200.0);
+    pc = fma(r2, pc, 1.0 / 479001600.0);
+    pc = fma(r2, pc, -1.0 / 3628800.0);
+    pc = fma(r2, pc, 1.0 / 40320.0);
+    pc = fma(r2, pc, -1.0 / 720.0);
+    pc = fma(r2, pc, 1.0 / 24.0);
+    pc = fma(r2, pc, -0.5);
+  } else {
+    ps = fmaf(r2, 1.f / 362880.f, -1.f / 5040.f);
+    ps = fmaf(r2, ps, 1.f / 120.f);
+    ps = fmaf(r2, ps, -1.f / 6.f);
+    pc = fmaf(r2, -1.f / 3628800.f, 1.f / 40320.f);
+    pc = fmaf(r2, pc, -1.f / 720.f);
+    pc = fmaf(r2, pc, 1.f / 24.f);
+    pc = fmaf(r2, pc, -0.5f);
+  }
+  const T sr = r + r * r2 * ps, cr = (T)1 + r2 * pc;
+  const int quadrant = (int)(k - 4.0 * rint(k * 0.25)) & 3;  // -2 .. 2
+  const T a = quadrant & 1 ? cr : sr, b = quadrant & 1 ? sr : cr;
+  s = quadrant & 2 ? -a : a;
+  c = (quadrant + 1) & 2 ? -b : b;
+}
+
+// The rotation of one position for a wave: the lane's (cos, sin) pairs, up to
+// four (half) or two (interleaved), times the plan's factor.
+template <typename T, bool ILV>
+struct LaneTurn {
+  static constexpr int N = ILV ? 2 : 4;
+  T c[N], s[N];
+
+  __device__ __forceinline__ void set(const RotaryPlan& p, double pos, int lane) {
+    T ct[2] = {}, st[2] = {};
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+      if (lane + 64 * k < p.half) {
+        turn<T>(pos * p.freq[lane + 64 * k], st[k], ct[k]);
+        ct[k] *= (T)p.factor;
+        st[k] *= (T)p.factor;
+      }
+    // first pair of the lane's columns
+    const int p0 = ILV ? 2 * lane : (4 * lane < p.half ? 4 * lane : 4 * lane - p.half);
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      c[e] = __shfl(ct[0], (p0 + e) & 63, 64);
+      s[e] = __shfl(st[0], (p0 + e) & 63, 64);
+      if (p.half > 64) {  // uniform
+        const T c1 = __shfl(ct[1], (p0 + e) & 63, 64), s1 = __shfl(st[1], (p0 + e) & 63, 64);
+        if (p0 + e >= 64) {
+          c[e] = c1;
+          s[e] = s1;
+        }
+      }
+    }
+  }
+
+  // Rotates the lane's columns y of a head.
+  __device__ __forceinline__ void apply(const RotaryPlan& p, T (&y)[4], int lane) const {
+    if constexpr (ILV) {
+      if (4 * lane < 2 * p.half) {
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const T a = y[2 * e], b = y[2 * e + 1];
+          y[2 * e] = a * c[e] - b * s[e];
+          y[2 * e + 1] = b * c[e] + a * s[e];
+        }
+      }
+    } else {
+      const bool lower = 4 * lane < p.half;
+      const int partner = lower ? lane + (p.half >> 2) : lane - (p.half >> 2);
+      T o[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] = __shfl(y[e], partner & 63, 64);
+      if (4 * lane < 2 * p.half) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = lower ? y[e] * c[e] - o[e] * s[e] : y[e] * c[e] + o[e] * s[e];
+      }
+    }
+  }
+};
+
+// Sum over a wave.
+template <typename T>
+__device__ __forceinline__ T wave_sum(T x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+  return x;
+}
+
+// RMS norm of a head with bf16 weights, in T.
+template <typename T>
+__device__ __forceinline__ void rms_norm(T (&y)[4], const uint16_t* w, double eps, int lane) {
+  const T ss = wave_sum<T>(y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3]);
+  T inv;
+  if constexpr (sizeof(T) == 8) inv = 1.0 / sqrt(ss / kHeadDim + eps);
+  else inv = 1.f / sqrtf(ss / (float)kHeadDim + (float)eps);
+  const ushort4 wb = *(const ushort4*)(w + 4 * lane);
+  y[0] = y[0] * inv * (T)bf16_to_f32(wb.x);
+  y[1] = y[1] * inv * (T)bf16_to_f32(wb.y);
+  y[2] = y[2] * inv * (T)bf16_to_f32(wb.z);
+  y[3] = y[3] * inv * (T)bf16_to_f32(wb.w);
+}
+
+// Four consecutive values of an f32, f16 or bf16 (uint16_t) row.
+struct bf16 { uint16_t bits; };
+__device__ __forceinline__ float4 load4(const float* p) { return *(const float4*)p; }
+__device__ __forceinline__ float4 load4(const _Float16* p) {
+  const f16x4 v = *(const f16x4*)p;
+  return {(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+__device__ __forceinline__ float4 load4(const bf16* p) {
+  const ushort4 v = *(const ushort4*)p;
+  return {bf16_to_f32(v.x), bf16_to_f32(v.y), bf16_to_f32(v.z), bf16_to_f32(v.w)};
+}
+__device__ __forceinline__ uint16_t f32_to_bf16(float x) {  // nearest, ties to even
+  const uint32_t u = __float_as_uint(x);
+  if (x != x) return (uint16_t)((u >> 16) | 0x40);
+  return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+}
+__device__ __forceinline__ void store4(float* p, const float (&y)[4]) {
+  *(float4*)p = float4{y[0], y[1], y[2], y[3]};
+}
+__device__ __forceinline__ void store4(_Float16* p, const float (&y)[4]) {
+  *(f16x4*)p = f16x4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+}
+__device__ __forceinline__ void store4(bf16* p, const float (&y)[4]) {
+  *(ushort4*)p = ushort4{f32_to_bf16(y[0]), f32_to_bf16(y[1]), f32_to_bf16(y[2]), f32_to_bf16(y[3])};
+}
+
+}  // namespace mi

@@ -1,0 +1,515 @@
+"""Rotary positions, and a paged KV cache in 4 bits for batches of sequences.
+
+A server of many sequences keeps their rows in pages of one pool per layer
+instead of one region each, and in 4 bits instead of 16 (288 bytes a row and KV
+head instead of 1024).  A layer of a step is
+
+    q = paged_append(pages, table, kv_len, k, v, rope=rope, cu_q=cu_q, q=q_proj,
+                     q_norm_w=qw, k_norm_w=kw)      # norm, rotation, append
+    o = attn_prefill_paged(pages, table, kv_len, cu_q, q, max_q, max_len, gate=gate)
+
+and of a decode step (one token per sequence) the same without cu_q, through
+attn_decode_paged.  The tables live on the device and the kernels read them, so
+a captured step follows them as the program updates them in place.
+
+PagedCache owns the pages of all layers and deals them to sequences;
+PagedCache.batch() makes the tables of a step.  The functions take tensors, so
+a program with an allocator of its own needs only the layout (include/mi_attn.h).
+
+Beside the single-sequence Cache / qk_norm_rope_append / attn_prefill and the
+ragged decode over whole regions (attention.py).  The reference keeps one f32
+cache for one sequence (src/cache.rs:45-128).
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .attention import HEAD_DIM, _ptr, _stream
+from .kv_cache import _cfg_get
+
+TILE_ROWS = 32
+TILE_BYTES = 9216
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class Rope:
+    """A rotation plan: frequencies (64 bits) of the first rotary_dim columns,
+    the layout of the pairs, and the factor on the rotated columns.
+
+    layout: "half" pairs columns (i, i + rotary_dim / 2), "interleaved" (2i, 2i + 1).
+    Without scaling, frequency i is theta^(-2i / rotary_dim).  scaling, a dict with
+    "type" and "factor" s (>= 1), stretches it for a context s times longer:
+      "linear"  every frequency / s
+      "ntk"     theta * s^(rotary_dim / (rotary_dim - 2)) in theta's place
+      "yarn"    by the turns r a pair makes over "original_max_position" rows:
+                frequency * (g + (1 - g) / s), g = (r - beta_slow) / (beta_fast - beta_slow)
+                held to [0, 1] ("beta_slow" 1, "beta_fast" 32), and the rotated columns
+                times "attention_factor" (default 0.1 ln s + 1)
+    frequencies: a sequence of rotary_dim / 2 numbers instead of all that."""
+
+    def __init__(self, rotary_dim: int = 64, theta: float = 1e7, layout: str = "half",
+                 scaling: dict | None = None, frequencies=None, factor: float | None = None):
+        rotary_dim = int(rotary_dim)
+        if rotary_dim < 0 or rotary_dim % 8 or rotary_dim > HEAD_DIM:
+            raise ValueError(f"rotary_dim {rotary_dim}: a multiple of 8, at most {HEAD_DIM}")
+        if layout not in ("half", "interleaved"):
+            raise ValueError(f"layout {layout!r}: 'half' or 'interleaved'")
+        turned = 1.0
+        if frequencies is None:
+            if not (theta > 0 and math.isfinite(theta)):
+                raise ValueError(f"theta {theta}")
+            frequencies, turned = _scaled(rotary_dim, float(theta), dict(scaling or {}))
+        elif scaling:
+            raise ValueError("frequencies are taken as they are: no scaling beside them")
+        f = [float(x) for x in frequencies]
+        if len(f) != rotary_dim // 2 or not all(math.isfinite(x) for x in f):
+            raise ValueError(f"{rotary_dim // 2} finite frequencies are wanted")
+        self.rotary_dim = rotary_dim
+        self.layout = layout
+        self.frequencies = tuple(f)
+        self.factor = float(turned if factor is None else factor)
+        if not math.isfinite(self.factor):
+            raise ValueError(f"factor {self.factor}")
+        self._f = (C.c_double * max(1, len(f)))(*f)
+        # the C arguments: frequencies, rotary_dim, interleaved, factor
+        self._args = (C.addressof(self._f), rotary_dim, int(layout == "interleaved"), self.factor)
+
+    @classmethod
+    def from_config(cls, config, layout: str = "half") -> "Rope":
+        """From a model's config.json dict: rope_theta, partial_rotary_factor,
+        rope_scaling ({"rope_type" or "type": ..., "factor": ...,
+        "original_max_position_embeddings": ...})."""
+        dim = int(round(float(_cfg_get(config, "partial_rotary_factor", 0.25)) *
+                        int(_cfg_get(config, "head_dim", HEAD_DIM))))
+        s = _cfg_get(config, "rope_scaling", None)
+        if s:
+            s = dict(s)
+            kind = s.pop("rope_type", None) or s.get("type", "default")
+            s["type"] = kind
+            if "original_max_position_embeddings" in s:
+                s["original_max_position"] = s.pop("original_max_position_embeddings")
+            if kind == "default":
+                s = None
+        return cls(dim, float(_cfg_get(config, "rope_theta", 1e7)), layout, s)
+
+
+def _scaled(dim: int, theta: float, scaling: dict):
+    """(frequencies, factor) of Rope's docstring."""
+    kind = scaling.pop("type", "none")
+    if kind == "none":
+        if scaling:
+            raise ValueError(f"scaling has no type but {sorted(scaling)}")
+        return [theta ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0
+    known = {"linear": set(), "ntk": set(),
+             "yarn": {"original_max_position", "beta_fast", "beta_slow", "attention_factor"}}
+    if kind not in known:
+        raise ValueError(f"scaling type {kind!r}: one of {sorted(known)}")
+    if "factor" not in scaling:
+        raise ValueError("scaling needs a factor")
+    s = float(scaling.pop("factor"))
+    if not (s >= 1.0 and math.isfinite(s)):
+        raise ValueError(f"scaling factor {s}: at least 1")
+    if set(scaling) - known[kind]:
+        raise ValueError(f"scaling {kind!r} does not know {sorted(set(scaling) - known[kind])}")
+    if kind == "ntk":
+        theta *= s ** (dim / (dim - 2.0))
+    f = [theta ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if kind == "linear":
+        return [x / s for x in f], 1.0
+    if kind == "ntk":
+        return f, 1.0
+    if "original_max_position" not in scaling:
+        raise ValueError("yarn needs original_max_position")
+    rows = float(scaling["original_max_position"])
+    slow, fast = float(scaling.get("beta_slow", 1.0)), float(scaling.get("beta_fast", 32.0))
+    if not (rows > 0 and fast > slow):
+        raise ValueError(f"yarn: original_max_position {rows}, beta_slow {slow}, beta_fast {fast}")
+    keep = [min(1.0, max(0.0, (rows * x / (2 * math.pi) - slow) / (fast - slow))) for x in f]
+    factor = scaling.get("attention_factor")
+    return ([x * (g + (1.0 - g) / s) for x, g in zip(f, keep)],
+            0.1 * math.log(s) + 1.0 if factor is None else float(factor))
+
+
+_NO_ROPE = Rope(0)
+
+
+# ----------------------------------------------------------------- checks --
+
+def _check_rows(name: str, t, n: int | None, heads: int | None, dtypes):
+    """[n, heads, 256] on the current device, its columns contiguous: (token
+    stride, head stride)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {[str(d) for d in dtypes]}, got {t.dtype}")
+    if t.dim() != 3 or t.shape[2] != HEAD_DIM:
+        raise ValueError(f"{name} must be [tokens, heads, {HEAD_DIM}], got {tuple(t.shape)}")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{name} has {t.shape[0]} tokens, expected {n}")
+    if heads is not None and t.shape[1] != heads:
+        raise ValueError(f"{name} has {t.shape[1]} heads, expected {heads}")
+    _check_device(name, t)
+    ts, hs, cs = t.stride()
+    if cs != 1:
+        raise ValueError(f"{name}: its {HEAD_DIM} columns must be contiguous")
+    if t.shape[1] == 1:
+        hs = HEAD_DIM
+    if t.shape[0] == 1:
+        ts = t.shape[1] * hs
+    size = t.element_size()
+    if (t.data_ptr() | ts * size | hs * size) & 15:
+        raise ValueError(f"{name}: every row must be 16-byte aligned")
+    if hs < HEAD_DIM or ts < HEAD_DIM:
+        raise ValueError(f"{name}: rows overlap (strides {ts}, {hs})")
+    return ts, hs
+
+
+def _check_device(name: str, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor, got {t.device}")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+
+
+def _check_table(name: str, t, numel: int | None, dtype=torch.int32) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    _check_device(name, t)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f"{name} has {t.numel()} elements, expected {numel}")
+
+
+def _check_pages(pages, block_table, kv_len, cu_q):
+    """The C arguments of the cache: pages .. batch; and the KV heads."""
+    _check_table("pages", pages, None, torch.uint8)
+    if pages.dim() != 4 or pages.shape[3] != TILE_BYTES or 0 in pages.shape:
+        raise ValueError(f"pages must be [pages, KV heads, page rows / {TILE_ROWS}, {TILE_BYTES}], "
+                         f"got {tuple(pages.shape)}")
+    _check_table("block_table", block_table, None)
+    if block_table.dim() != 2 or 0 in block_table.shape:
+        raise ValueError(f"block_table must be [batch, pages of a sequence], got "
+                         f"{tuple(block_table.shape)}")
+    batch = block_table.shape[0]
+    _check_table("kv_len", kv_len, batch)
+    if cu_q is not None:
+        _check_table("cu_q", cu_q, batch + 1)
+    return (pages.data_ptr(), pages.shape[0], pages.shape[2] * TILE_ROWS, block_table.data_ptr(),
+            block_table.shape[1], kv_len.data_ptr(), _ptr(cu_q), batch), pages.shape[1]
+
+
+def _check_norm(name: str, w) -> None:
+    if w is not None:
+        _check_table(name, w, HEAD_DIM, torch.bfloat16)
+        if w.data_ptr() & 15:
+            raise ValueError(f"{name} must be 16-byte aligned")
+
+
+def _check_out(name: str, out, n: int, heads: int, dtype, device):
+    if out is None:
+        return torch.empty((n, heads, HEAD_DIM), dtype=dtype, device=device)
+    _check_table(name, out, n * heads * HEAD_DIM, dtype)
+    if out.data_ptr() & 15:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    return out
+
+
+# -------------------------------------------------------------- operators --
+
+def rope_apply(x: torch.Tensor, positions: torch.Tensor, rope: Rope,
+               norm_w: torch.Tensor | None = None, eps: float = 1e-6,
+               out: torch.Tensor | None = None, out_dtype=None) -> torch.Tensor:
+    """x [n, heads, 256] (f32, f16 or bf16, any token and head stride) rotated
+    at positions [n] (int32 or int64), after an RMS norm with norm_w (bf16 [256])
+    if given.  Returns [n, heads, 256] of out_dtype (default x's); out may be x."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3:
+        raise TypeError("x must be a tensor [tokens, heads, 256]")
+    n, heads = x.shape[0], x.shape[1]
+    ts, hs = _check_rows("x", x, None, None, _DTYPES)
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be an int32 or int64 tensor")
+    _check_table("positions", positions, n, positions.dtype)
+    if not isinstance(rope, Rope):
+        raise TypeError("rope must be a Rope")
+    _check_norm("norm_w", norm_w)
+    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    if dtype not in _DTYPES:
+        raise TypeError(f"out_dtype {dtype}")
+    out = _check_out("out", out, n, heads, dtype, x.device)
+    _lib.check(_lib.lib().mi_rope_apply(
+        x.data_ptr(), _DTYPES[x.dtype], ts, hs, n, heads, HEAD_DIM, positions.data_ptr(),
+        positions.dtype == torch.int64, _ptr(norm_w), eps, *rope._args, out.data_ptr(),
+        _DTYPES[dtype], _stream()))
+    return out
+
+
+def paged_append(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+                 k: torch.Tensor, v: torch.Tensor, rope: Rope | None = None,
+                 cu_q: torch.Tensor | None = None, q: torch.Tensor | None = None,
+                 q_norm_w: torch.Tensor | None = None, k_norm_w: torch.Tensor | None = None,
+                 eps: float = 1e-6, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Appends n tokens' k, v [n, G, 256] as the last rows of their sequences:
+    K normed (k_norm_w) and rotated at its row, both quantised to 4 bits.  kv_len
+    counts the rows after the call; token i of sequence s (cu_q[s] + i) is row
+    kv_len[s] - tokens of s + i; without cu_q each sequence brings one token.
+    With q [n, H, 256] returns it normed and rotated, [n, H, 256] f16 (q_out; may
+    be q).  q, k, v: one of f32, f16, bf16, any token and head stride (a view of a
+    projection).  No rope: no rotation."""
+    head, G = _check_pages(pages, block_table, kv_len, cu_q)
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise TypeError("k must be a tensor [tokens, KV heads, 256]")
+    n, batch = k.shape[0], head[-1]
+    if cu_q is None and n != batch:
+        raise ValueError(f"{n} tokens for {batch} sequences without cu_q")
+    kts, khs = _check_rows("k", k, None, G, _DTYPES)
+    vts, vhs = _check_rows("v", v, n, G, (k.dtype,))
+    _check_norm("q_norm_w", q_norm_w)
+    _check_norm("k_norm_w", k_norm_w)
+    rope = _NO_ROPE if rope is None else rope
+    if not isinstance(rope, Rope):
+        raise TypeError("rope must be a Rope")
+    H = qts = qhs = 0
+    if q is not None:
+        qts, qhs = _check_rows("q", q, n, None, (k.dtype,))
+        H = q.shape[1]
+        q_out = _check_out("q_out", q_out, n, H, torch.float16, q.device)
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _lib.check(_lib.lib().mi_paged_append(
+        *head, n, H, G, HEAD_DIM, _DTYPES[k.dtype], _ptr(q), qts, qhs, k.data_ptr(), kts, khs,
+        v.data_ptr(), vts, vhs, _ptr(q_norm_w), _ptr(k_norm_w), eps, *rope._args, _ptr(q_out),
+        _stream()))
+    return q_out
+
+
+def paged_read(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+               cu_q: torch.Tensor | None = None, n: int | None = None,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """(k, v), each [n, G, 256] f16: the last cu_q[s + 1] - cu_q[s] rows of each
+    sequence (without cu_q the last row), as stored.  n: their number, cu_q[-1];
+    with cu_q it must be given, so that the call need not wait for the GPU."""
+    head, G = _check_pages(pages, block_table, kv_len, cu_q)
+    if n is None:
+        if cu_q is not None:
+            raise ValueError("n must be given with cu_q")
+        n = head[-1]
+    n = int(n)
+    k, v = out if out is not None else (None, None)
+    k = _check_out("k", k, n, G, torch.float16, pages.device)
+    v = _check_out("v", v, n, G, torch.float16, pages.device)
+    _lib.check(_lib.lib().mi_paged_read(*head, n, G, HEAD_DIM, k.data_ptr(), v.data_ptr(), _stream()))
+    return k, v
+
+
+def paged_workspace(batch: int, n: int, max_q: int, max_len: int, num_q_heads: int = 16,
+                    num_kv_heads: int = 2, device="cuda") -> torch.Tensor:
+    """Workspace of attn_decode_paged / attn_prefill_paged for steps of these
+    sizes (n tokens in all, at most max_q and max_len rows a sequence)."""
+    nbytes = _lib.lib().mi_attn_paged_workspace_size(batch, n, max_q, max_len, num_q_heads,
+                                                     num_kv_heads)
+    if not nbytes:
+        raise ValueError(f"no workspace for batch {batch}, {n} tokens, max_q {max_q}, max_len "
+                         f"{max_len}, heads {num_q_heads} / {num_kv_heads}")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _attend(pages, block_table, kv_len, cu_q, q, max_q, max_len, gate, out, workspace):
+    head, G = _check_pages(pages, block_table, kv_len, cu_q)
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise TypeError("q must be a tensor [tokens, heads, 256]")
+    n, H = q.shape[0], q.shape[1]
+    if cu_q is None and n != head[-1]:
+        raise ValueError(f"{n} tokens for {head[-1]} sequences")
+    qts, qhs = _check_rows("q", q, None, None, (torch.float16,))
+    if H % G:
+        raise ValueError(f"{H} query heads for {G} KV heads")
+    g_type = gts = ghs = 0
+    if gate is not None:
+        gts, ghs = _check_rows("gate", gate, n, H, (torch.float16, torch.float32))
+        g_type = _DTYPES[gate.dtype]
+    out = _check_out("out", out, n, H, torch.float16, q.device)
+    if workspace is None:
+        workspace = paged_workspace(head[-1], n, max_q, max_len, H, G, q.device)
+    else:
+        _check_table("workspace", workspace, None, torch.uint8)
+    _lib.check(_lib.lib().mi_attn_paged(
+        *head, n, max_q, max_len, H, G, HEAD_DIM, q.data_ptr(), qts, qhs, _ptr(gate), g_type, gts,
+        ghs, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream()))
+    return out
+
+
+def attn_decode_paged(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+                      q: torch.Tensor, max_len: int, gate: torch.Tensor | None = None,
+                      out: torch.Tensor | None = None,
+                      workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """A decode step: q [batch, H, 256] f16, sequence s over its kv_len[s] rows
+    (at most max_len).  gate [batch, H, 256] f16 or f32: out *= sigmoid(gate).  An
+    empty sequence gives zeros.  out may be q or gate itself."""
+    return _attend(pages, block_table, kv_len, None, q, 1, int(max_len), gate, out, workspace)
+
+
+def attn_prefill_paged(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Tensor,
+                       cu_q: torch.Tensor, q: torch.Tensor, max_q: int, max_len: int,
+                       gate: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                       workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of a ragged batch, its rows already appended: q [n, H, 256]
+    f16, tokens cu_q[s] .. cu_q[s + 1] - 1 the last rows of sequence s (at most
+    max_q tokens and max_len rows).  Prompts, chunks behind cached rows, drafts to
+    verify.  gate and out as for attn_decode_paged."""
+    if cu_q is None:
+        raise TypeError("cu_q must be a torch.Tensor")
+    return _attend(pages, block_table, kv_len, cu_q, q, int(max_q), int(max_len), gate, out, workspace)
+
+
+# -------------------------------------------------------------- the cache --
+
+@dataclass
+class PagedBatch:
+    """The tables of one step, for every layer: PagedCache.batch()."""
+    block_table: torch.Tensor     # int32 [batch, pages]
+    kv_len: torch.Tensor          # int32 [batch]
+    cu_q: torch.Tensor | None     # int32 [batch + 1]; None: one token each
+    positions: torch.Tensor       # int32 [n], the row of every token
+    n: int
+    max_q: int
+    max_len: int
+
+
+class PagedCache:
+    """Pages of every full-attention layer, dealt to sequences.
+
+    Sequences are numbers that add() gives.  extend(seq, n) makes room for n more
+    rows, truncate(seq, rows) takes a rejected draft back (rows past it stay in
+    place and are overwritten), remove(seq) gives its pages back.  A page number
+    means the same rows in every layer.  Not thread-safe, like Cache."""
+
+    def __init__(self, config=None, *, num_layers: int | None = None, num_q_heads: int = 16,
+                 num_kv_heads: int = 2, head_dim: int = HEAD_DIM, num_pages: int = 256,
+                 page_rows: int = 64, device="cuda"):
+        from .kv_cache import FULL_ATTN_INTERVAL
+        n_hidden = int(_cfg_get(config, "num_hidden_layers", num_layers or 1))
+        self.num_q_heads = int(_cfg_get(config, "num_attention_heads", num_q_heads))
+        self.num_kv_heads = int(_cfg_get(config, "num_key_value_heads", num_kv_heads))
+        if int(_cfg_get(config, "head_dim", head_dim)) != HEAD_DIM:
+            raise ValueError(f"head_dim must be {HEAD_DIM}")
+        if self.num_kv_heads <= 0 or self.num_q_heads % self.num_kv_heads:
+            raise ValueError(f"{self.num_q_heads} query heads for {self.num_kv_heads} KV heads")
+        if page_rows < TILE_ROWS or page_rows > 1024 or page_rows & (page_rows - 1):
+            raise ValueError(f"page_rows {page_rows}: a power of two, 32 to 1024")
+        if num_pages <= 0:
+            raise ValueError(f"num_pages {num_pages}")
+        linear = (_cfg_get(config, "linear_num_value_heads", 0) or 0) > 0 and \
+                 (_cfg_get(config, "linear_num_key_heads", 0) or 0) > 0
+        self.full_layers = [i for i in range(n_hidden)
+                            if not linear or (i + 1) % FULL_ATTN_INTERVAL == 0]
+        self.page_rows = int(page_rows)
+        self.num_pages = int(num_pages)
+        self.device = torch.device(device)
+        # zeros: a fresh page's rows are 0 * code + 0
+        self._pages = {layer: torch.zeros((self.num_pages, self.num_kv_heads,
+                                           self.page_rows // TILE_ROWS, TILE_BYTES),
+                                          dtype=torch.uint8, device=self.device)
+                       for layer in self.full_layers}
+        self._free = list(range(self.num_pages - 1, -1, -1))
+        self._rows: dict[int, int] = {}
+        self._table: dict[int, list[int]] = {}
+        self._next = 0
+
+    def pages(self, layer: int) -> torch.Tensor:
+        """The pages of model layer `layer`."""
+        try:
+            return self._pages[layer]
+        except KeyError:
+            raise ValueError(f"layer {layer} is not a full-attention layer") from None
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def add(self) -> int:
+        seq = self._next
+        self._next += 1
+        self._rows[seq], self._table[seq] = 0, []
+        return seq
+
+    def _known(self, seq: int) -> None:
+        if seq not in self._rows:
+            raise ValueError(f"no sequence {seq}")
+
+    def len(self, seq: int) -> int:
+        self._known(seq)
+        return self._rows[seq]
+
+    def extend(self, seq: int, rows: int) -> int:
+        """Room for `rows` more rows; the sequence's rows.  Takes nothing where
+        the free pages do not suffice (MemoryError)."""
+        self._known(seq)
+        if rows < 0:
+            raise ValueError(f"rows {rows}")
+        total = self._rows[seq] + rows
+        need = -(-total // self.page_rows) - len(self._table[seq])
+        if need > len(self._free):
+            raise MemoryError(f"{need} pages wanted, {len(self._free)} of {self.num_pages} free")
+        for _ in range(need):
+            self._table[seq].append(self._free.pop())
+        self._rows[seq] = total
+        return total
+
+    def truncate(self, seq: int, rows: int) -> None:
+        self._known(seq)
+        if not 0 <= rows <= self._rows[seq]:
+            raise ValueError(f"{rows} rows of a sequence of {self._rows[seq]}")
+        keep = -(-rows // self.page_rows)
+        self._free.extend(reversed(self._table[seq][keep:]))
+        del self._table[seq][keep:]
+        self._rows[seq] = rows
+
+    def remove(self, seq: int) -> None:
+        self.truncate(seq, 0)
+        del self._rows[seq], self._table[seq]
+
+    def batch(self, seqs, new=1) -> PagedBatch:
+        """Extends each of seqs by its new rows (a number for all, or one each)
+        and makes the step's tables.  All of them or, on an error, none."""
+        seqs = list(seqs)
+        counts = [int(new)] * len(seqs) if isinstance(new, int) else [int(x) for x in new]
+        if not seqs or len(counts) != len(seqs) or len(set(seqs)) != len(seqs):
+            raise ValueError("a batch is one or more different sequences, each with its new rows")
+        for s, c in zip(seqs, counts):
+            self._known(s)
+            if c < 0:
+                raise ValueError(f"rows {c}")
+        if not sum(counts):
+            raise ValueError("no sequence has a new row")
+        before = [self._rows[s] for s in seqs]
+        try:
+            for s, c in zip(seqs, counts):
+                self.extend(s, c)
+        except MemoryError:
+            for s, b in zip(seqs, before):
+                self.truncate(s, b)
+            raise
+        n, B = sum(counts), len(seqs)
+        M = max(1, max(len(self._table[s]) for s in seqs))
+        host = [i for s in seqs for i in self._table[s] + [-1] * (M - len(self._table[s]))]
+        host += [self._rows[s] for s in seqs]
+        at = [0]
+        for c in counts:
+            at.append(at[-1] + c)
+        host += at
+        for b, c in zip(before, counts):
+            host += range(b, b + c)
+        # one copy for all of the step's tables
+        t = torch.tensor(host, dtype=torch.int32).to(self.device)
+        table, kv_len, cu_q, positions = t.split([B * M, B, B + 1, n])
+        return PagedBatch(table.view(B, M), kv_len, None if all(c == 1 for c in counts) else cu_q,
+                          positions, n, max(counts), max(self._rows[s] for s in seqs))
