@@ -36,6 +36,12 @@ constexpr int kQuantGroup = 64;
 constexpr int kPageRowsMin = 32, kPageRowsMax = 1024;
 constexpr int kPagedRatioMax = 16;  // query heads per KV head
 
+// A load through the scalar cache of a table that no kernel writes while it is
+// read; the address is the same for the whole wave.
+__device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+
 // The pages of one layer and the rows of a batch of sequences in them.
 struct PagedView {
   uint8_t* pages;
@@ -45,16 +51,19 @@ struct PagedView {
   int64_t num_pages;
   int32_t cols, page_shift, batch, G;
 
-  // Base of tile t (32-row index) of sequence s and KV head h; null where the
-  // table has no such page.
-  __device__ __forceinline__ uint8_t* tile(int s, int h, int t) const {
-    const int pt = page_shift - 5;  // tiles per page, as a shift
-    const int j = t >> pt;
-    if (j >= cols) return nullptr;
-    const int32_t id = table[(int64_t)s * cols + j];
+  // Page of tile t (32-row index) of sequence s, the same for a whole wave; -1
+  // past the table.
+  __device__ __forceinline__ int32_t page(int s, int t) const {
+    const int j = t >> (page_shift - 5);
+    return j < cols ? uniform_load(table + (int64_t)s * cols + j) : -1;
+  }
+  // Base of tile t of KV head h in page id; null where the pool has no such page.
+  __device__ __forceinline__ uint8_t* at(int32_t id, int h, int t) const {
     if (id < 0 || id >= num_pages) return nullptr;
+    const int pt = page_shift - 5;  // tiles per page, as a shift
     return pages + (((int64_t)id * G + h) * ((int64_t)1 << pt) + (t & ((1 << pt) - 1))) * kTileBytes;
   }
+  __device__ __forceinline__ uint8_t* tile(int s, int h, int t) const { return at(page(s, t), h, t); }
   // Tokens [q0, q0 + nq) of the call belong to sequence s (nq may be <= 0 for
   // a table that does not ascend; tokens are bounded by n in the kernels).
   __device__ __forceinline__ void tokens(int s, int& q0, int& nq) const {
@@ -69,12 +78,19 @@ mi_status paged_view(void* pages, int64_t num_pages, int32_t page_rows, const in
                      int32_t num_kv_heads, int32_t head_dim, PagedView* out);
 
 // A pair of codes of word w, its nibbles k (low half) and k + 4 (high half),
-// as 16 + code in f16.
+// as 16 + code in f16.  `sixteens` is 0x4c004c00 in a vector register
+// (mi::sixteens()): and-or is one instruction only if no more than one of its
+// operands is a constant or a scalar register.
 template <int K>
-__device__ __forceinline__ f16x2 codes16(uint32_t w) {
+__device__ __forceinline__ f16x2 codes16(uint32_t w, uint32_t sixteens) {
   constexpr int sh = 6 - 4 * K;
   const uint32_t x = sh >= 0 ? w << (sh & 31) : w >> (-sh & 31);
-  return __builtin_bit_cast(f16x2, (x & 0x03c003c0u) | 0x4c004c00u);
+  return __builtin_bit_cast(f16x2, (x & 0x03c003c0u) | sixteens);
+}
+__device__ __forceinline__ uint32_t sixteens() {
+  uint32_t v;
+  asm("v_mov_b32 %0, 0x4c004c00" : "=v"(v));
+  return v;
 }
 
 __device__ __forceinline__ f16x2 pk_fma(f16x2 a, f16x2 b, f16x2 c) {
@@ -83,17 +99,20 @@ __device__ __forceinline__ f16x2 pk_fma(f16x2 a, f16x2 b, f16x2 c) {
 
 // Eight values of one scale and offset, in the order {0,4,1,5,2,6,3,7} of the
 // word's nibbles.
-__device__ __forceinline__ f16x8 dequant_row(uint32_t w, f16x2 scale, f16x2 offset) {
-  const f16x2 a = pk_fma(codes16<0>(w), scale, offset), b = pk_fma(codes16<1>(w), scale, offset);
-  const f16x2 c = pk_fma(codes16<2>(w), scale, offset), d = pk_fma(codes16<3>(w), scale, offset);
+__device__ __forceinline__ f16x8 dequant_row(uint32_t w, f16x2 scale, f16x2 offset,
+                                             uint32_t x16) {
+  const f16x2 a = pk_fma(codes16<0>(w, x16), scale, offset);
+  const f16x2 b = pk_fma(codes16<1>(w, x16), scale, offset);
+  const f16x2 c = pk_fma(codes16<2>(w, x16), scale, offset);
+  const f16x2 d = pk_fma(codes16<3>(w, x16), scale, offset);
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 // Eight keys of one V column; scale, offset: in the same order {0,4,1,5,..}.
-__device__ __forceinline__ f16x8 dequant_col(uint32_t w, f16x8 s, f16x8 o) {
-  const f16x2 a = pk_fma(codes16<0>(w), f16x2{s[0], s[1]}, f16x2{o[0], o[1]});
-  const f16x2 b = pk_fma(codes16<1>(w), f16x2{s[2], s[3]}, f16x2{o[2], o[3]});
-  const f16x2 c = pk_fma(codes16<2>(w), f16x2{s[4], s[5]}, f16x2{o[4], o[5]});
-  const f16x2 d = pk_fma(codes16<3>(w), f16x2{s[6], s[7]}, f16x2{o[6], o[7]});
+__device__ __forceinline__ f16x8 dequant_col(uint32_t w, f16x8 s, f16x8 o, uint32_t x16) {
+  const f16x2 a = pk_fma(codes16<0>(w, x16), f16x2{s[0], s[1]}, f16x2{o[0], o[1]});
+  const f16x2 b = pk_fma(codes16<1>(w, x16), f16x2{s[2], s[3]}, f16x2{o[2], o[3]});
+  const f16x2 c = pk_fma(codes16<2>(w, x16), f16x2{s[4], s[5]}, f16x2{o[4], o[5]});
+  const f16x2 d = pk_fma(codes16<3>(w, x16), f16x2{s[6], s[7]}, f16x2{o[6], o[7]});
   return f16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 

@@ -3,7 +3,7 @@
 //
 // The columns of a (sequence, KV head) are its (token, query head of the
 // group) pairs, token-major; a workgroup takes CT blocks of 16 of them and a
-// range of 32-row tiles, which its four waves take in turn.  A wave's tile:
+// range of 32-row tiles, which its waves take in turn.  A wave's tile:
 //   S [32 keys x 16 CT] = K Q^T    16x16x32 MFMA, K dequantised in registers
 //   running maximum and sum per column (f32), P = 2^(S - max) in f16
 //   O^T [256 x 16 CT] += V^T P     V dequantised in registers
@@ -11,6 +11,9 @@
 // operand layout of P, so nothing goes through LDS between the products.  K of
 // the next tile is loaded into K's registers while P V runs, V into V's while
 // K Q^T runs.
+//
+// A workgroup's waves join through LDS, workgroups that share an item through
+// partials that paged_merge_kernel joins.
 #include <algorithm>
 #include <cmath>
 
@@ -20,8 +23,12 @@ namespace {
 
 constexpr int D = mi::kHeadDim;
 constexpr float kNegBig = -1e30f;
-constexpr int kWaves = 4;
 constexpr int kColPitch = D + 4;  // f32 per column of the merge buffer
+
+// Waves of a workgroup: two to a SIMD where the accumulators leave room.
+constexpr int waves(int ct) { return ct == 1 ? 8 : 4; }
+// Tiles below which a workgroup is not split further: one to a wave.
+constexpr int kMinTiles = 8;
 
 struct AttnArgs {
   mi::PagedView pv;
@@ -30,148 +37,175 @@ struct AttnArgs {
   const void* gate;  // f16, or f32 (gate32), or null
   int64_t g_ts, g_hs;
   _Float16* out;     // [n][G R][D]
-  float* part_o;     // [item][split][16 CT][D]
-  float* part_ml;    // [item][split][16 CT][2]
-  int32_t n, R, max_q, max_len, splits, ncb, gate32;
+  float* part_o;     // [2 workgroups][16 CT][D]
+  float* part_ml;    // [2 workgroups][16 CT][2]
+  int2* seg;         // [batch G ncb]: first slot and last workgroup of an item, or -1
+  int32_t n, R, max_q, max_len, wgs, ncb, gate32, dsplit;
 };
 
-// One item: a block of columns of a sequence and KV head.
-struct Item {
-  int s, h, q0, nq, len;
-  int c0;       // first column
-  int ntiles;   // tiles that some column of it sees
-  bool bad;     // beyond max_q or max_len
+// A sequence as its work: ncb blocks of 16 CT columns per KV head, each over
+// ntiles tiles of 32 rows.  Items of a sequence are (KV head, block); its weight,
+// items times tiles over the KV heads, is ncb * ntiles.
+struct Seq {
+  int q0, nq, len, ncb, ntiles;
+  bool bad;  // beyond max_q or max_len
 };
-
-template <int CT>
-__device__ __forceinline__ Item get_item(const AttnArgs& a, int64_t item) {
-  Item it;
-  const int cb = (int)(item % a.ncb);
-  const int64_t sh = item / a.ncb;
-  it.s = (int)(sh / a.pv.G);
-  it.h = (int)(sh - (int64_t)it.s * a.pv.G);
-  a.pv.tokens(it.s, it.q0, it.nq);
-  it.len = a.pv.kv_len[it.s];
-  it.bad = it.len < 0 || it.len > a.max_len || it.nq > a.max_q;
-  if (it.nq <= 0 || it.q0 < 0 || (int64_t)it.q0 + it.nq > a.n) it.nq = 0;
-  it.c0 = cb * 16 * CT;
-  const int last = min(it.nq - 1, (it.c0 + 16 * CT - 1) / a.R);
-  const int end = it.len - it.nq + last + 1;
-  it.ntiles = it.bad || it.c0 >= it.nq * a.R || end <= 0 ? 0 : (end + 31) / 32;
-  return it;
+template <int CT, bool UNIFORM>
+__device__ __forceinline__ Seq get_seq(const AttnArgs& a, int s) {
+  auto load = [](const int32_t* p) { return UNIFORM ? mi::uniform_load(p) : *p; };
+  Seq r;
+  r.q0 = a.pv.cu_q ? load(a.pv.cu_q + s) : s;
+  r.nq = a.pv.cu_q ? load(a.pv.cu_q + s + 1) - r.q0 : 1;
+  r.len = load(a.pv.kv_len + s);
+  r.bad = r.len < 0 || r.len > a.max_len || r.nq > a.max_q;
+  if (r.nq <= 0 || r.q0 < 0 || (int64_t)r.q0 + r.nq > a.n) r.nq = 0;
+  r.ncb = r.bad ? 0 : (r.nq * a.R + 16 * CT - 1) / (16 * CT);
+  r.ntiles = r.bad ? 0 : (r.len + 31) >> 5;
+  return r;
 }
 
-// out of one value: the gate, then f16.
-__device__ __forceinline__ void put(const AttnArgs& a, int64_t tok, int head, int d, float x) {
+// out of four columns: the gate, then f16.
+__device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
   if (a.gate) {
     const int64_t gi = tok * a.g_ts + head * a.g_hs + d;
-    x = mi::gate_mul(x, a.gate32 ? ((const float*)a.gate)[gi] : (float)((const _Float16*)a.gate)[gi]);
+    f32x4 g;
+    if (a.gate32) {
+      g = *(const f32x4*)((const float*)a.gate + gi);
+    } else {
+      const f16x4 h = *(const f16x4*)((const _Float16*)a.gate + gi);
+      g = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = mi::gate_mul(x[e], g[e]);
   }
-  a.out[(tok * a.pv.G * a.R + head) * D + d] = (_Float16)x;
+  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * D + d) =
+      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
 }
 
-template <int CT>
-__global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) paged_attn_kernel(const AttnArgs a) {
-  extern __shared__ float lds[];
-  // merge buffer [wave][16][kColPitch], maxima and sums [wave][16 CT][2], and
-  // for CT > 1 the Q operands [CT][8][64] of 16 bytes
-  float* const mbuf = lds;
-  float* const mlbuf = lds + kWaves * 16 * kColPitch;
-  f16x8* const qbuf = (f16x8*)(mlbuf + kWaves * 16 * CT * 2);
+// Sum over the workgroup and the exclusive prefix of each thread's x.
+template <int NT>
+__device__ __forceinline__ int block_scan(int x, int& before, int* lds) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int run = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(run, d, 64);
+    if (lane >= d) run += y;
+  }
+  __syncthreads();  // lds may hold an earlier scan's
+  if (lane == 63) lds[w] = run;
+  __syncthreads();
+  int base = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) {
+    if (i < w) base += lds[i];
+    total += lds[i];
+  }
+  before = base + run - x;
+  return __builtin_amdgcn_readfirstlane(total);
+}
 
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int m16 = lane & 15, quad = lane >> 4;
-  const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  const int64_t item = bid / a.splits;
-  const int split = (int)(bid - item * a.splits);
-  if (item >= (int64_t)a.pv.batch * a.pv.G * a.ncb) return;
-  const Item it = get_item<CT>(a, item);
-  if (it.bad) {  // every token of the sequence, by its first workgroup
-    if (it.c0 == 0 && split == 0)
-      for (int64_t i = threadIdx.x; i < (int64_t)it.nq * a.R * D; i += 256) {
-        const int64_t tok = it.q0 + i / (a.R * D);
-        a.out[(tok * a.pv.G + it.h) * a.R * D + i % (a.R * D)] = (_Float16)__builtin_nanf("");
-      }
+// The sequence s that holds weight unit `unit(total weight)` of weight(s), and the
+// weight before it; s = 0 where no sequence does.  (The host holds the tiles of a
+// batch, over KV heads and blocks, below 2^31.)
+template <int NT, typename W, typename F>
+__device__ __forceinline__ void find_seq(int batch, W weight, F unit, int& s, int& before) {
+  __shared__ int lds[NT / 64 + 2];
+  const int t = threadIdx.x;
+  s = 0;
+  before = 0;
+  if (batch == 1) {
+    unit(__builtin_amdgcn_readfirstlane(weight(0)));
     return;
   }
-  const int ncols = it.nq * a.R;
-  if (it.c0 >= ncols) return;
-  const int t0 = (int)((int64_t)it.ntiles * split / a.splits);
-  const int t1 = (int)((int64_t)it.ntiles * (split + 1) / a.splits);
-  if (t0 == t1 && a.splits > 1) return;
-
-  // the lane's columns: their rows of Q, and the rows they see
-  int lim[CT];
-  f16x8 q1[8];  // CT == 1: the Q operands
-#pragma unroll
-  for (int ct = 0; ct < CT; ct++) {
-    const int c = it.c0 + 16 * ct + m16;
-    const bool in = c < ncols;
-    const int tok = in ? c / a.R : 0, head = it.h * a.R + (in ? c - tok * a.R : 0);
-    lim[ct] = in ? it.len - it.nq + tok + 1 : 0;
-    const _Float16* qp = a.q + (it.q0 + tok) * a.q_ts + head * a.q_hs + 16 * quad;
-    if (CT == 1 || w == ct % kWaves) {
-#pragma unroll
-      for (int f = 0; f < 8; f++) {  // group f / 2, step f % 2
-        f16x8 x = {};
-        if (in) x = *(const f16x8*)(qp + 64 * (f >> 1) + 8 * (f & 1));
-        x = f16x8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
-        if constexpr (CT == 1) q1[f] = x;
-        else qbuf[(ct * 8 + f) * 64 + lane] = x;
+  int total = 0, pre = 0, x = 0;
+  for (int c = 0; c < batch; c += NT) {
+    x = c + t < batch ? weight(c + t) : 0;
+    total += block_scan<NT>(x, pre, lds);
+  }
+  const int want = unit(total);
+  if (want >= total) return;
+  int base = 0;
+  for (int c = 0; c < batch; c += NT) {
+    if (batch > NT) {  // one pass of a small batch has them already
+      x = c + t < batch ? weight(c + t) : 0;
+      const int sum = block_scan<NT>(x, pre, lds);
+      if (want >= base + sum) {  // uniform
+        base += sum;
+        continue;
       }
     }
+    if (base + pre <= want && want < base + pre + x) {
+      lds[NT / 64] = c + t;
+      lds[NT / 64 + 1] = base + pre;
+    }
+    break;
   }
-  if constexpr (CT > 1) __syncthreads();
-  const int lim0 = it.len - it.nq + it.c0 / a.R + 1;                                 // first column's
-  const int lim1 = it.len - it.nq + min(it.nq - 1, (it.c0 + 16 * CT - 1) / a.R) + 1;  // last column's
+  __syncthreads();
+  s = __builtin_amdgcn_readfirstlane(lds[NT / 64]);
+  before = __builtin_amdgcn_readfirstlane(lds[NT / 64 + 1]);
+}
 
-  const float c2 = mi::kLog2e / 16.f;  // softmax scale 1 / sqrt(256), in base 2
+// Eight columns of Q in dequant_row's order.
+__device__ __forceinline__ f16x8 in_order(f16x8 x) {
+  return f16x8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+}
+
+// One wave's state over the tiles of an item.
+template <int CT>
+struct Wave {
   f32x4 o[CT][16];
   float m[CT], l[CT];
-#pragma unroll
-  for (int ct = 0; ct < CT; ct++) {
-    m[ct] = kNegBig;
-    l[ct] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; i++) o[ct][i] = f32x4{};
-  }
   u32x4 k[4], v[4];
   f16x8 ks[2], vs[4], vo[4];
-  auto load_k = [&](const uint8_t* p) {
+  int lim[CT];  // rows that the lane's columns see
+  uint32_t x16;
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < 4; i++) k[i] = ((const u32x4*)p)[64 * i + lane];
+    for (int ct = 0; ct < CT; ct++) {
+      m[ct] = kNegBig;
+      l[ct] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; i++) ks[i] = ((const f16x8*)(p + mi::kKScale))[16 * i + m16];
-  };
-  auto load_v = [&](const uint8_t* p) {
+      for (int i = 0; i < 16; i++) o[ct][i] = f32x4{};
+    }
+  }
+  // A tile as a buffer of its size, or of none: then the loads below return zeros
+  // and move nothing, so the last tile of a wave prefetches without a branch
+  // (whose two ways would need the loaded registers copied, and waited for).
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, p ? mi::kTileBytes : 0,
+                                             0x00020000);
+  }
+  static __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t b, int lane_at, int at) {
+    return __builtin_amdgcn_raw_buffer_load_b128(b, lane_at + at, 0, 0);
+  }
+  __device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t b, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = ((const u32x4*)(p + mi::kVCodes))[64 * i + lane];
+    for (int i = 0; i < 4; i++) k[i] = load(b, 16 * lane, 1024 * i);
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+      ks[i] = __builtin_bit_cast(f16x8, load(b, 16 * (lane & 15), mi::kKScale + 256 * i));
+  }
+  __device__ __forceinline__ void load_v(__amdgpu_buffer_rsrc_t b, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = load(b, 16 * lane, mi::kVCodes + 1024 * i);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      vs[i] = ((const f16x8*)(p + mi::kVScale))[2 * (4 * i + quad)];
-      vo[i] = ((const f16x8*)(p + mi::kVScale))[2 * (4 * i + quad) + 1];
+      vs[i] = __builtin_bit_cast(f16x8, load(b, 32 * (lane >> 4), mi::kVScale + 128 * i));
+      vo[i] = __builtin_bit_cast(f16x8, load(b, 32 * (lane >> 4), mi::kVScale + 128 * i + 16));
     }
-  };
-  bool lost = false;  // a page of the range is not there
-  int t = t0 + w;
-  const uint8_t* cur = t < t1 ? a.pv.tile(it.s, it.h, t) : nullptr;
-  const uint8_t* next = t + kWaves < t1 ? a.pv.tile(it.s, it.h, t + kWaves) : nullptr;
-  if (cur) {
-    load_k(cur);
-    load_v(cur);
   }
-  for (; t < t1; t += kWaves) {
-    const uint8_t* after = t + 2 * kWaves < t1 ? a.pv.tile(it.s, it.h, t + 2 * kWaves) : nullptr;
-    if (!cur) {
-      lost = true;
-      if (next) {
-        load_k(next);
-        load_v(next);
-      }
-      cur = next;
-      next = after;
-      continue;
-    }
+
+  // One tile, rows row0 .. row0 + 31; `next` (or null) is loaded on the way.
+  // MASKED: some column does not see some row; lim1: rows that some column sees.
+  template <bool MASKED, typename Q>
+  __device__ __forceinline__ void tile(__amdgpu_buffer_rsrc_t next, int row0, int lim1, int lane, Q q) {
+    const int quad = lane >> 4;
+    // the words as they are here: without this, their shifts move up to the loads,
+    // three registers more for each
+#pragma unroll
+    for (int i = 0; i < 4; i++) asm volatile("" : "+v"(k[i]));
     f32x4 sc[CT][2];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) sc[ct][0] = sc[ct][1] = f32x4{};
@@ -183,21 +217,19 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) paged_attn_kernel(const 
       for (int sub = 0; sub < 2; sub++)
         ka[sub] = mi::dequant_row(k[2 * sub + (g >> 1)][2 * (g & 1) + step],
                                   f16x2{ks[sub][2 * g], ks[sub][2 * g]},
-                                  f16x2{ks[sub][2 * g + 1], ks[sub][2 * g + 1]});
+                                  f16x2{ks[sub][2 * g + 1], ks[sub][2 * g + 1]}, x16);
 #pragma unroll
       for (int ct = 0; ct < CT; ct++) {
-        f16x8 qf;
-        if constexpr (CT == 1) qf = q1[f];
-        else qf = qbuf[(ct * 8 + f) * 64 + lane];
+        const f16x8 qf = q(ct, f);
 #pragma unroll
         for (int sub = 0; sub < 2; sub++)
           sc[ct][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[sub], qf, sc[ct][sub], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);  // a few operands at a time
     }
-    if (next) load_k(next);
-    const int row0 = 32 * t;
+    load_k(next, lane);
     uint32_t poison[CT] = {};  // groups whose values a column must take for not a number
-    if (row0 + 32 > lim0) {    // some column does not see some row (uniform)
+    if constexpr (MASKED) {
       // Keys out of sight weigh nothing whatever they hold: their scores are
       // replaced, and V, whose MFMA would make NaN of 0 * NaN, is cleared where
       // no column sees the row or where it is not finite; columns that do see
@@ -209,22 +241,46 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) paged_attn_kernel(const 
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (row0 + 16 * sub + 4 * quad + i >= lim[ct]) sc[ct][sub][i] = -__builtin_inff();
+      // in pairs of rows (4 quad + i, 16 more), as the scales lie
+      auto seen = [&](int i, int end) {
+        const int r = row0 + 4 * quad + i;
+        return (r < end ? 0xffffu : 0u) | (r + 16 < end ? 0xffff0000u : 0u);
+      };
+      uint32_t odd = 0;  // halves whose exponent is all ones carry into bit 15
 #pragma unroll
-      for (int g = 0; g < 4; g++)
+      for (int g = 0; g < 4; g++) {
+        u32x4 ws = __builtin_bit_cast(u32x4, vs[g]), wo = __builtin_bit_cast(u32x4, vo[g]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const int row = row0 + 16 * (e & 1) + 4 * quad + (e >> 1);
-          const bool odd = !(__builtin_fabsf16(vs[g][e]) < (_Float16)__builtin_inff()) ||
-                           !(__builtin_fabsf16(vo[g][e]) < (_Float16)__builtin_inff());
-          if (odd || row >= lim1) {
+        for (int i = 0; i < 4; i++) {
+          ws[i] &= seen(i, lim1);
+          wo[i] &= seen(i, lim1);
+          odd |= ((ws[i] & 0x7c007c00u) + 0x04000400u) | ((wo[i] & 0x7c007c00u) + 0x04000400u);
+        }
+        vs[g] = __builtin_bit_cast(f16x8, ws);
+        vo[g] = __builtin_bit_cast(f16x8, wo);
+      }
+      if (__any((odd & 0x80008000u) != 0)) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          u32x4 ws = __builtin_bit_cast(u32x4, vs[g]), wo = __builtin_bit_cast(u32x4, vo[g]);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t top =
+                (((ws[i] & 0x7c007c00u) + 0x04000400u) | ((wo[i] & 0x7c007c00u) + 0x04000400u)) &
+                0x80008000u;
+            const uint32_t halves = (top >> 15) * 0xffffu;
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
-              if (odd && row < lim[ct]) poison[ct] |= 1u << g;
-            vs[g][e] = (_Float16)0.f;
-            vo[g][e] = (_Float16)0.f;
+              if (halves & seen(i, lim[ct])) poison[ct] |= 1u << g;
+            ws[i] &= ~halves;
+            wo[i] &= ~halves;
           }
+          vs[g] = __builtin_bit_cast(f16x8, ws);
+          vo[g] = __builtin_bit_cast(f16x8, wo);
         }
+      }
     }
+    constexpr float c2 = mi::kLog2e / 16.f;  // softmax scale 1 / sqrt(256), in base 2
     f16x8 p[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
@@ -235,9 +291,10 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) paged_attn_kernel(const 
         top = fmaxf(top, x[e]);
       }
       top = mi::max_rows(top);
-      const float mn = fmaxf(m[ct], top);
-      if (__any(mn > m[ct])) {
-        const float f = __builtin_amdgcn_exp2f(m[ct] - mn);
+      // The reference point moves only when weights would pass 2^8 (f16 holds
+      // them to 2^15, the sums are f32), so after the first tile hardly ever.
+      if (__any(top > m[ct] + 8.f)) {
+        const float mn = fmaxf(m[ct], top), f = __builtin_amdgcn_exp2f(m[ct] - mn);
         l[ct] *= f;
 #pragma unroll
         for (int i = 0; i < 16; i++) o[ct][i] *= f;
@@ -245,22 +302,25 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) paged_attn_kernel(const 
       }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const float y = __builtin_amdgcn_exp2f(x[e] - mn);
+        const float y = __builtin_amdgcn_exp2f(x[e] - m[ct]);
         l[ct] += y;
         p[ct][e] = (_Float16)y;  // the MFMA's operand: off by 2^-11 of itself at most
       }
     }
 #pragma unroll
-    for (int g = 0; g < 4; g++)
+    for (int g = 0; g < 4; g++) {
+      asm volatile("" : "+v"(v[g]));
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const f16x8 va = mi::dequant_col(v[g][j], vs[g], vo[g]);
+        const f16x8 va = mi::dequant_col(v[g][j], vs[g], vo[g], x16);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
           o[ct][4 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[ct], o[ct][4 * g + j], 0, 0, 0);
       }
-    if (next) load_v(next);
-    if (row0 + 32 > lim0) {
+      __builtin_amdgcn_sched_barrier(0);  // not all sixteen operands at once
+    }
+    load_v(next, lane);
+    if constexpr (MASKED) {
 #pragma unroll
       for (int ct = 0; ct < CT; ct++)
         if (__any(poison[ct] != 0)) {
@@ -271,103 +331,309 @@ __global__ void __launch_bounds__(256, CT == 1 ? 2 : 1) paged_attn_kernel(const 
             if (all >> (i >> 2) & 1) o[ct][i] += __builtin_nanf("");
         }
     }
-    cur = next;
-    next = after;
   }
+};
 
-  // the waves' maxima and sums, then their O by 16 columns
-#pragma unroll
-  for (int ct = 0; ct < CT; ct++) {
-    l[ct] = mi::sum_rows(l[ct]);
-    if (lost) l[ct] = __builtin_nanf("");
-    if (quad == 0) {
-      float* const ml = mlbuf + ((w * CT + ct) * 16 + m16) * 2;
-      ml[0] = m[ct];
-      ml[1] = l[ct];
+template <int CT>
+__global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_kernel(const AttnArgs a) {
+  constexpr int NW = waves(CT), NT = 64 * NW;
+  extern __shared__ float lds[];
+  // maxima [wave][16 CT], sums [wave][16], largest maxima [16]; for CT > 1 the Q
+  // operands [CT][8][64] of 16 bytes; merge buffer [wave][min(16, columns)][kColPitch]
+  float* const mbox = lds;
+  float* const lbox = mbox + NW * 16 * CT;
+  float* const tbox = lbox + NW * 16;
+  f16x8* const qbuf = (f16x8*)(tbox + 16);
+  float* const mbuf = (float*)(qbuf + (CT > 1 ? CT * 8 * 64 : 0));
+  const int mcols = min(16, a.max_q * a.R);
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int bid = blockIdx.x;
+
+  // By chunks: every item in chunks of up to kMinTiles tiles, one to a workgroup,
+  // where the grid has that many.  Else a flat line of tiles, [sequence][KV
+  // head][block][tile], in even pieces, one to a workgroup.
+  int s, before, f = 0, f1 = 0;
+  const int G = a.pv.G;
+  bool chunks = true;
+  auto parts = [](int ntiles) { return (ntiles + kMinTiles - 1) / kMinTiles; };
+  find_seq<NT>(
+      a.pv.batch,
+      [&](int i) {
+        const Seq q = get_seq<CT, false>(a, i);
+        return q.ncb * parts(q.ntiles);
+      },
+      [&](int total) {
+        chunks = (uint32_t)total * G <= (uint32_t)a.wgs;
+        f = bid;
+        f1 = min(bid + 1, total * G);
+        return chunks ? (int)((uint32_t)f / (uint32_t)G) : total;
+      },
+      s, before);
+  if (!chunks)
+    find_seq<NT>(
+        a.pv.batch,
+        [&](int i) {
+          const Seq q = get_seq<CT, false>(a, i);
+          return q.ncb * q.ntiles;
+        },
+        [&](int total) {
+          const uint32_t all = (uint32_t)total * G, each = all / a.wgs, more = all - each * a.wgs;
+          f = (int)(each * bid + min((uint32_t)bid, more));
+          f1 = f + (int)each + ((uint32_t)bid < more);
+          return (int)((uint32_t)f / (uint32_t)G);
+        },
+        s, before);
+  if (f >= f1) return;
+  int slot = 2 * bid;
+
+  Wave<CT> st;
+  st.x16 = mi::sixteens();
+  while (f < f1) {
+    const Seq sq = get_seq<CT, true>(a, s);
+    const int per = chunks ? parts(sq.ntiles) : sq.ntiles, weight = sq.ncb * per;
+    if (f >= G * (before + weight)) {
+      before += weight;
+      s++;
+      continue;
     }
-  }
-  __syncthreads();
-  const int64_t slot = (item * a.splits + split) * (16 * CT);
+    const uint32_t local = f - G * before, vh = local / (uint32_t)per, at = local - vh * per;
+    const int h = (int)(vh / (uint32_t)sq.ncb), cb = (int)vh - h * sq.ncb;
+    int t0, t1;
+    if (chunks) {
+      t0 = (int)(at * (uint32_t)sq.ntiles / (uint32_t)per);
+      t1 = (int)((at + 1) * (uint32_t)sq.ntiles / (uint32_t)per);
+      f = f1;
+    } else {
+      t0 = (int)at;
+      t1 = min(sq.ntiles, t0 + (f1 - f));
+      f += t1 - t0;
+    }
+    const int c0 = cb * 16 * CT, ncols = sq.nq * a.R, first = sq.len - sq.nq;
+
+    // the lane's columns: their rows of Q, and the rows they see (columns past the
+    // last take the first's, which nothing reads)
+    f16x8 q1[8];  // CT == 1: the Q operands
 #pragma unroll
-  for (int ct = 0; ct < CT; ct++) {
-    float top = kNegBig;
+    for (int ct = 0; ct < CT; ct++) {
+      const int c = c0 + 16 * ct + (lane & 15);
+      const bool in = c < ncols;
+      const int tok = in ? c / a.R : 0, head = h * a.R + (in ? c - tok * a.R : 0);
+      st.lim[ct] = in ? first + tok + 1 : 0;
+      const _Float16* qp = a.q + (sq.q0 + tok) * a.q_ts + head * a.q_hs + 16 * (lane >> 4);
+      if (CT == 1 || w == ct % NW) {
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) top = fmaxf(top, mlbuf[((i * CT + ct) * 16 + m16) * 2]);
-    const float f = __builtin_amdgcn_exp2f(m[ct] - top);
-    float* const mb = mbuf + (w * 16 + m16) * kColPitch + 16 * quad;
-#pragma unroll
-    for (int g = 0; g < 4; g++)
-#pragma unroll
-      for (int i = 0; i < 4; i++)  // columns 64 g + 16 quad + 4 i + j of O
-        *(f32x4*)(mb + 64 * g + 4 * i) =
-            f32x4{o[ct][4 * g][i], o[ct][4 * g + 1][i], o[ct][4 * g + 2][i], o[ct][4 * g + 3][i]} * f;
-    __syncthreads();
-    const int d = threadIdx.x;
-    for (int c = 0; c < 16; c++) {
-      const int col = it.c0 + 16 * ct + c;
-      if (col >= ncols) break;
-      float top_c = kNegBig, sum = 0.f, x = 0.f;
-#pragma unroll
-      for (int i = 0; i < kWaves; i++) top_c = fmaxf(top_c, mlbuf[((i * CT + ct) * 16 + c) * 2]);
-#pragma unroll
-      for (int i = 0; i < kWaves; i++) {
-        const float* const ml = mlbuf + ((i * CT + ct) * 16 + c) * 2;
-        sum += ml[1] * __builtin_amdgcn_exp2f(ml[0] - top_c);
-        x += mbuf[(i * 16 + c) * kColPitch + d];
-      }
-      if (a.splits == 1) {
-        const int tok = col / a.R;
-        put(a, it.q0 + tok, it.h * a.R + col - tok * a.R, d, sum == 0.f ? 0.f : x / sum);
-      } else {
-        a.part_o[(slot + 16 * ct + c) * D + d] = x;
-        if (d == 0) {
-          a.part_ml[(slot + 16 * ct + c) * 2] = top_c;
-          a.part_ml[(slot + 16 * ct + c) * 2 + 1] = sum;
+        for (int i = 0; i < 8; i++) {  // group i / 2, step i % 2
+          const f16x8 x = *(const f16x8*)(qp + 64 * (i >> 1) + 8 * (i & 1));
+          if constexpr (CT == 1) q1[i] = x;
+          else qbuf[(ct * 8 + i) * 64 + lane] = in_order(x);
         }
       }
     }
-    if (ct + 1 < CT) __syncthreads();
+    if constexpr (CT > 1) __syncthreads();
+    auto q = [&](int ct, int i) {
+      if constexpr (CT == 1) return q1[i];
+      else return qbuf[(ct * 8 + i) * 64 + lane];
+    };
+    const int lim0 = first + c0 / a.R + 1;                                       // first column's
+    const int lim1 = first + min(sq.nq - 1, (c0 + 16 * CT - 1) / a.R) + 1;       // last column's
+    // tiles [t0, tm) are seen whole, [tm, t1) not
+    const int tm = max(t0, min(t1, lim0 >> 5));
+
+    st.clear();
+    // A page that is not there is read as no bytes and the sums become not a
+    // number.  Pages are looked up two tiles ahead, loads issued one ahead.
+    bool lost = false;
+    auto base = [&](int32_t id, int t) -> const uint8_t* {
+      if (t >= t1) return nullptr;
+      const uint8_t* p = a.pv.at(id, h, t);
+      lost = lost || !p;
+      return p;
+    };
+    auto page = [&](int t) { return t < t1 ? a.pv.page(s, t) : -1; };
+    int t = t0 + w;
+    if (t < t1) {
+      const int32_t id0 = page(t), id1 = page(t + NW);
+      const auto cur = st.buffer(base(id0, t));
+      st.load_k(cur, lane);
+      st.load_v(cur, lane);
+      if constexpr (CT == 1) {  // behind the tile's loads: it waits for Q's
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 8; i++) q1[i] = in_order(q1[i]);
+      }
+      const uint8_t* next = base(id1, t + NW);
+      for (; t < tm; t += NW) {
+        const int32_t id = page(t + 2 * NW);
+        st.template tile<false>(st.buffer(next), 32 * t, lim1, lane, q);
+        next = base(id, t + 2 * NW);
+      }
+      for (; t < t1; t += NW) {
+        const int32_t id = page(t + 2 * NW);
+        st.template tile<true>(st.buffer(next), 32 * t, lim1, lane, q);
+        next = base(id, t + 2 * NW);
+      }
+    }
+
+    // The waves' maxima, then their sums and O relative to the largest, 16 columns
+    // at a time; a thread joins four output columns.
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      st.l[ct] = mi::sum_rows(st.l[ct]);
+      if (lost) st.l[ct] = __builtin_nanf("");
+      if (lane < 16) mbox[(w * CT + ct) * 16 + lane] = st.m[ct];
+    }
+    // from here on the lane's addresses are formed anew: hoisted out of the loop
+    // over items they would be spilled across the tiles
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int m16 = tid & 15, quad = (tid >> 4) & 3;
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == sq.ntiles;
+    const int64_t col0 = (int64_t)slot * (16 * CT);
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      float top = kNegBig;
+#pragma unroll
+      for (int i = 0; i < NW; i++) top = fmaxf(top, mbox[(i * CT + ct) * 16 + m16]);
+      const float scale = __builtin_amdgcn_exp2f(st.m[ct] - top);
+      if (quad == 0) {
+        lbox[w * 16 + m16] = st.l[ct] * scale;
+        tbox[m16] = top;  // the same from every wave
+      }
+      float* const mb = mbuf + (w * mcols + m16) * kColPitch + 16 * quad;
+      if (m16 < mcols) {
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)  // columns 64 g + 16 quad + 4 i + j of O
+            *(f32x4*)(mb + 64 * g + 4 * i) = f32x4{st.o[ct][4 * g][i], st.o[ct][4 * g + 1][i],
+                                                   st.o[ct][4 * g + 2][i], st.o[ct][4 * g + 3][i]} *
+                                             scale;
+      }
+      __syncthreads();
+      const int d = 4 * (tid & 63);
+      for (int c = w; c < mcols; c += NW) {
+        const int col = c0 + 16 * ct + c;
+        if (col >= ncols) break;
+        float sum = 0.f;
+        f32x4 x = {};
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+          sum += lbox[i * 16 + c];
+          x += *(const f32x4*)(mbuf + (i * mcols + c) * kColPitch + d);
+        }
+        if (whole) {
+          const int tok = col / a.R;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, x * inv);
+        } else {
+          *(f32x4*)(a.part_o + (col0 + 16 * ct + c) * D + d) = x;
+          if (d == 0) *(float2*)(a.part_ml + (col0 + 16 * ct + c) * 2) = float2{tbox[c], sum};
+        }
+      }
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) {  // where the merge finds the item's pieces
+      int2* const sg = a.seg + ((int64_t)s * G + h) * a.ncb + cb;
+      if (whole) {
+        sg->x = -1;
+      } else {
+        if (t0 == 0) sg->x = slot;
+        if (t1 == sq.ntiles) sg->y = bid;
+      }
+    }
+    slot = 2 * bid + 1;  // only the first and the last item of a workgroup are not whole
   }
 }
 
-// Joins the splits of an item: a workgroup per (item, column), a thread per
-// output column.
+// Joins the pieces of an item: a workgroup per (item, column, part of the 256
+// output columns); its first piece is in slot seg.x, the others in slot 2 x of the
+// workgroups x behind.  Items without rows become zero, those beyond max_q or
+// max_len NaN.
 template <int CT>
-__global__ void __launch_bounds__(D) paged_merge_kernel(const AttnArgs a) {
-  const int64_t bid = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  const int64_t item = bid / (16 * CT);
-  const int c = (int)(bid - item * (16 * CT)), d = threadIdx.x;
-  if (item >= (int64_t)a.pv.batch * a.pv.G * a.ncb) return;
-  const Item it = get_item<CT>(a, item);
-  if (it.bad || it.c0 + c >= it.nq * a.R) return;
-  float top = kNegBig, sum = 0.f, x = 0.f;
-  for (int i = 0; i < a.splits; i++) {
-    const int t0 = (int)((int64_t)it.ntiles * i / a.splits);
-    const int t1 = (int)((int64_t)it.ntiles * (i + 1) / a.splits);
-    if (t0 == t1) continue;
-    const int64_t slot = (item * a.splits + i) * (16 * CT) + c;
-    const float mi_ = a.part_ml[slot * 2], li = a.part_ml[slot * 2 + 1];
-    const float xi = a.part_o[slot * D + d];
-    const float mn = fmaxf(top, mi_), f = __builtin_amdgcn_exp2f(top - mn),
-                g = __builtin_amdgcn_exp2f(mi_ - mn);
-    sum = sum * f + li * g;
-    x = x * f + xi * g;
-    top = mn;
+__global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
+  __shared__ f32x4 acc[256];
+  __shared__ float ml[256][2];
+  const uint32_t parts = a.dsplit, d4 = 64 / parts, groups = 256 / d4;
+  const uint32_t bid = blockIdx.y * gridDim.x + blockIdx.x;  // below 2^31 (make_plan)
+  const uint32_t ic = bid / parts, part = bid - ic * parts;
+  const uint32_t item = ic / (16 * CT), c = ic % (16 * CT);
+  if (item >= (uint32_t)a.pv.batch * a.pv.G * a.ncb) return;
+  const uint32_t sh = item / a.ncb, cb = item - sh * a.ncb;
+  const int s = sh / a.pv.G, h = sh - s * a.pv.G;
+  const Seq sq = get_seq<CT, true>(a, s);
+  const int col = cb * 16 * CT + c;
+  const uint32_t t = threadIdx.x, lane4 = t % d4, grp = t / d4, d = 4 * (part * d4 + lane4);
+  if (sq.bad || sq.ntiles == 0) {  // every token of the sequence, by its items' first workgroups
+    if (cb || c || part) return;
+    const _Float16 x = sq.bad ? (_Float16)__builtin_nanf("") : (_Float16)0.f;
+    const int width = a.R * D;
+    for (int tok = 0; tok < sq.nq; tok++)
+      for (int i = t; i < width; i += 256)
+        a.out[((int64_t)(sq.q0 + tok) * a.pv.G + h) * width + i] = x;
+    return;
   }
-  const int col = it.c0 + c, tok = col / a.R;
-  put(a, it.q0 + tok, it.h * a.R + col - tok * a.R, d, sum == 0.f ? 0.f : x / sum);
+  if (col >= sq.nq * a.R) return;
+  const int2 sg = a.seg[item];
+  if (sg.x < 0) return;
+  const int first = sg.x >> 1, count = sg.y - first + 1;
+  auto slot = [&](int i) { return (i ? 2 * (first + i) : sg.x) * (16 * CT) + (int)c; };
+  float top = kNegBig, sum = 0.f;
+  f32x4 x = {};
+  for (int i0 = grp; i0 < count; i0 += 4 * (int)groups) {
+    float mi_[4], li[4];
+    f32x4 xi[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int i = i0 + u * (int)groups;
+      const bool in = i < count;
+      const int sl = slot(in ? i : i0);
+      mi_[u] = in ? a.part_ml[sl * 2] : kNegBig;
+      li[u] = in ? a.part_ml[sl * 2 + 1] : 0.f;
+      xi[u] = *(const f32x4*)(a.part_o + (int64_t)sl * D + d);
+    }
+    const float mn = fmaxf(top, fmaxf(fmaxf(mi_[0], mi_[1]), fmaxf(mi_[2], mi_[3])));
+    const float f = __builtin_amdgcn_exp2f(top - mn);
+    sum *= f;
+    x *= f;
+    top = mn;
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      if (i0 + u * (int)groups >= count) continue;
+      const float g = __builtin_amdgcn_exp2f(mi_[u] - mn);
+      sum += li[u] * g;
+      x += xi[u] * g;
+    }
+  }
+  acc[t] = x;
+  if (lane4 == 0) {
+    ml[grp][0] = top;
+    ml[grp][1] = sum;
+  }
+  __syncthreads();
+  if (t >= d4) return;  // a thread per four output columns of the part
+  const int used = min((int)groups, count);
+  float m = kNegBig, total = 0.f;
+  f32x4 y = {};
+  for (int g = 0; g < used; g++) m = fmaxf(m, ml[g][0]);
+  for (int g = 0; g < used; g++) {
+    const float f = __builtin_amdgcn_exp2f(ml[g][0] - m);
+    total += ml[g][1] * f;
+    y += acc[g * d4 + t] * f;
+  }
+  const int tok = col / a.R;
+  put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y * (total == 0.f ? 0.f : 1.f / total));
 }
 
-// Column blocks of 16 a workgroup takes: those of one sequence's tokens, up to 4.
-int column_blocks(int32_t max_q, int R) {
-  const int64_t cols = (int64_t)max_q * R;
-  return cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-}
+// Column blocks of 16 a workgroup takes: 2 where a sequence has more than one.
+int column_blocks(int32_t max_q, int R) { return (int64_t)max_q * R <= 16 ? 1 : 2; }
 
 struct Plan {
-  int ct, ncb, splits;
-  int64_t items;
-  size_t o_bytes, ml_bytes;
+  int ct, ncb, wgs, dsplit;
+  int64_t items, tiles;
+  size_t o_bytes, ml_bytes, seg_bytes;
+  size_t bytes() const { return o_bytes + ml_bytes + seg_bytes; }
 };
 
 Plan make_plan(int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
@@ -376,29 +642,30 @@ Plan make_plan(int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
   p.ct = column_blocks(max_q, R);
   p.ncb = (int)(((int64_t)max_q * R + 16 * p.ct - 1) / (16 * p.ct));
   p.items = (int64_t)batch * G * p.ncb;
-  const int64_t tiles = std::max<int64_t>(1, ((int64_t)max_len + 31) / 32);
-  const int64_t want = (1024 + p.items - 1) / p.items;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({want, (tiles + 7) / 8, 256}));
-  const int64_t cols = p.splits > 1 ? p.items * p.splits * 16 * p.ct : 0;
+  p.tiles = p.items * (((int64_t)max_len + 31) / 32);
+  const int64_t per_item = (((int64_t)max_len + 31) / 32 + kMinTiles - 1) / kMinTiles;
+  p.wgs = (int)std::max<int64_t>(1, std::min<int64_t>(256, p.items * per_item));
+  p.dsplit = p.items * std::min(16 * p.ct, max_q * R) <= 256 ? 4 : 1;
+  if (p.items * 16 * p.ct * p.dsplit > INT32_MAX) p.tiles = INT32_MAX;  // refused
+  const int64_t cols = (int64_t)2 * p.wgs * 16 * p.ct;
   p.o_bytes = cols * D * sizeof(float);
   p.ml_bytes = cols * 2 * sizeof(float);
+  p.seg_bytes = (p.items * sizeof(int2) + 15) & ~(size_t)15;
   return p;
 }
 
 template <int CT>
-mi_status run(const AttnArgs& a, const Plan& p, hipStream_t s) {
+mi_status run(AttnArgs& a, const Plan& p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
-  const int lds = (kWaves * 16 * kColPitch + kWaves * 16 * CT * 2) * (int)sizeof(float) +
-                  (CT > 1 ? CT * 8 * 64 * 16 : 0);
-  MI_TRY(mi::set_lds_limit((const void*)paged_attn_kernel<CT>, lds, done));
-  const int64_t wgs = p.items * p.splits, gx = std::min<int64_t>(wgs, 1 << 22);
-  MI_HIP(mi::launch("paged_attn", paged_attn_kernel<CT>,
-                    dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)), dim3(256), lds, s, a));
-  if (p.splits > 1) {
-    const int64_t ms = p.items * 16 * CT, mx = std::min<int64_t>(ms, 1 << 22);
-    MI_HIP(mi::launch("paged_merge", paged_merge_kernel<CT>,
-                      dim3((unsigned)mx, (unsigned)((ms + mx - 1) / mx)), dim3(D), 0, s, a));
-  }
+  constexpr int NW = waves(CT);
+  const int fixed = (NW * 16 * (CT + 1) + 16) * (int)sizeof(float) + (CT > 1 ? CT * 8 * 64 * 16 : 0);
+  const int per_col = NW * kColPitch * (int)sizeof(float);
+  MI_TRY(mi::set_lds_limit((const void*)paged_attn_kernel<CT>, fixed + 16 * per_col, done));
+  MI_HIP(mi::launch("paged_attn", paged_attn_kernel<CT>, dim3((unsigned)p.wgs), dim3(64 * NW),
+                    fixed + std::min(16, a.max_q * a.R) * per_col, s, a));
+  const int64_t ms = p.items * 16 * CT * p.dsplit, mx = std::min<int64_t>(ms, 1 << 22);
+  MI_HIP(mi::launch("paged_merge", paged_merge_kernel<CT>,
+                    dim3((unsigned)mx, (unsigned)((ms + mx - 1) / mx)), dim3(256), 0, s, a));
   return MI_OK;
 }
 
@@ -421,7 +688,8 @@ extern "C" size_t mi_attn_paged_workspace_size(int32_t batch, int32_t n, int32_t
       max_len < 0)
     return 0;
   const Plan p = make_plan(batch, std::min(max_q, n), max_len, num_q_heads, num_kv_heads);
-  return std::max<size_t>(256, p.o_bytes + p.ml_bytes);
+  if (p.tiles >= INT32_MAX) return 0;
+  return p.bytes();
 }
 
 extern "C" mi_status mi_attn_paged(
@@ -458,9 +726,12 @@ extern "C" mi_status mi_attn_paged(
   }
   max_q = std::min(max_q, n);
   const Plan p = make_plan(batch, max_q, max_len, num_q_heads, num_kv_heads);
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.o_bytes + p.ml_bytes)
+  if (p.tiles >= INT32_MAX)
+    return mi::fail(MI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d rows in one call", batch, max_q,
+                    max_len);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes())
     return mi::fail(MI_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes,
-                    p.o_bytes + p.ml_bytes);
+                    p.bytes());
   a.q = (const _Float16*)q;
   a.q_ts = q_token_stride;
   a.q_hs = q_head_stride;
@@ -475,8 +746,10 @@ extern "C" mi_status mi_attn_paged(
   a.R = num_q_heads / num_kv_heads;
   a.max_q = max_q;
   a.max_len = max_len;
-  a.splits = p.splits;
+  a.seg = (int2*)((char*)workspace + p.o_bytes + p.ml_bytes);
+  a.wgs = p.wgs;
   a.ncb = p.ncb;
+  a.dsplit = p.dsplit;
   const hipStream_t s = (hipStream_t)stream;
-  return p.ct == 1 ? run<1>(a, p, s) : p.ct == 2 ? run<2>(a, p, s) : run<4>(a, p, s);
+  return p.ct == 1 ? run<1>(a, p, s) : run<2>(a, p, s);
 }

@@ -375,13 +375,14 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const ReadArgs a) {
     return;
   }
   const int c = t & 31;  // columns 8 c .. 8 c + 7
+  const uint32_t x16 = mi::sixteens();
   if (t < 128) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       const int r = 4 * i + (t >> 5);
       const uint32_t wd = ((const uint32_t*)tile)[k_word(r, c)];
       const f16x2 so = ((const f16x2*)(tile + mi::kKScale))[4 * r + (c >> 3)];
-      const f16x8 y = mi::dequant_row(wd, f16x2{so[0], so[0]}, f16x2{so[1], so[1]});
+      const f16x8 y = mi::dequant_row(wd, f16x2{so[0], so[0]}, f16x2{so[1], so[1]}, x16);
       if (r >= r0 && r < r1) *out(a.k, r, c) = f16x8{y[0], y[2], y[4], y[6], y[1], y[3], y[5], y[7]};
     }
   } else {
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(256) paged_read_kernel(const ReadArgs a) {
     const f16x8 s = sp[0], o = sp[1];
     f16x8 col[8];  // column e of the eight rows, in dequant_col's order
 #pragma unroll
-    for (int e = 0; e < 8; e++) col[e] = mi::dequant_col(e < 4 ? w0[e] : w1[e - 4], s, o);
+    for (int e = 0; e < 8; e++) col[e] = mi::dequant_col(e < 4 ? w0[e] : w1[e - 4], s, o, x16);
 #pragma unroll
     for (int p = 0; p < 8; p++) {  // element p: row 16 (p % 2) + 4 quad + p / 2
       const int r = 16 * (p & 1) + 4 * quad + (p >> 1);
