@@ -1,0 +1,115 @@
+// What the kernels of attention over the paged 4-bit cache share: their
+// arguments, the walk over a ragged batch, the output.
+#pragma once
+
+#include "paged.h"
+
+namespace mi {
+
+constexpr float kNegBig = -1e30f;  // below every score's base-2 exponent
+
+struct AttnArgs {
+  PagedView pv;
+  const _Float16* q;
+  int64_t q_ts, q_hs;
+  const void* gate;  // f16, or f32 (gate32), or null
+  int64_t g_ts, g_hs;
+  _Float16* out;     // [n][G R][D]
+  float* part_o;     // [2 workgroups][16 CT][D]
+  float* part_ml;    // [2 workgroups][16 CT][2]
+  int2* seg;         // [batch G ncb]: first slot and last workgroup of an item, or -1
+  int32_t n, R, max_q, max_len, wgs, ncb, gate32, dsplit;
+};
+
+// out of four columns: the gate, then f16.
+__device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
+  if (a.gate) {
+    const int64_t gi = tok * a.g_ts + head * a.g_hs + d;
+    f32x4 g;
+    if (a.gate32) {
+      g = *(const f32x4*)((const float*)a.gate + gi);
+    } else {
+      const f16x4 h = *(const f16x4*)((const _Float16*)a.gate + gi);
+      g = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] = gate_mul(x[e], g[e]);
+  }
+  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * kHeadDim + d) =
+      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+}
+
+// Sum over the workgroup and the exclusive prefix of each thread's x.
+template <int NT>
+__device__ __forceinline__ int block_scan(int x, int& before, int* lds) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int run = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(run, d, 64);
+    if (lane >= d) run += y;
+  }
+  __syncthreads();  // lds may hold an earlier scan's
+  if (lane == 63) lds[w] = run;
+  __syncthreads();
+  int base = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) {
+    if (i < w) base += lds[i];
+    total += lds[i];
+  }
+  before = base + run - x;
+  return __builtin_amdgcn_readfirstlane(total);
+}
+
+// The sequence s that holds weight unit `unit(total weight)` of weight(s), and the
+// weight before it; s = 0 where no sequence does.  (The host holds the tiles of a
+// batch, over KV heads and blocks, below 2^31.)
+template <int NT, typename W, typename F>
+__device__ __forceinline__ void find_seq(int batch, W weight, F unit, int& s, int& before) {
+  __shared__ int lds[NT / 64 + 2];
+  const int t = threadIdx.x;
+  s = 0;
+  before = 0;
+  if (batch == 1) {
+    unit(__builtin_amdgcn_readfirstlane(weight(0)));
+    return;
+  }
+  int total = 0, pre = 0, x = 0;
+  for (int c = 0; c < batch; c += NT) {
+    x = c + t < batch ? weight(c + t) : 0;
+    total += block_scan<NT>(x, pre, lds);
+  }
+  const int want = unit(total);
+  if (want >= total) return;
+  int base = 0;
+  for (int c = 0; c < batch; c += NT) {
+    if (batch > NT) {  // one pass of a small batch has them already
+      x = c + t < batch ? weight(c + t) : 0;
+      const int sum = block_scan<NT>(x, pre, lds);
+      if (want >= base + sum) {  // uniform
+        base += sum;
+        continue;
+      }
+    }
+    if (base + pre <= want && want < base + pre + x) {
+      lds[NT / 64] = c + t;
+      lds[NT / 64 + 1] = base + pre;
+    }
+    break;
+  }
+  __syncthreads();
+  s = __builtin_amdgcn_readfirstlane(lds[NT / 64]);
+  before = __builtin_amdgcn_readfirstlane(lds[NT / 64 + 1]);
+}
+
+// Eight columns of Q in dequant_row's order.
+__device__ __forceinline__ f16x8 in_order(f16x8 x) {
+  return f16x8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
+}
+
+// The prompts' form (paged_prefill.hip): workspace bytes, and the launches.
+size_t paged_prefill_workspace(int32_t batch, int32_t n, int32_t max_q, int32_t max_len, int H, int G);
+mi_status paged_prefill(AttnArgs& a, void* workspace, hipStream_t s);
+
+}  // namespace mi

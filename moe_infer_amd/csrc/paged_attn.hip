@@ -17,31 +17,20 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged.h"
+#include "paged_attn.h"
 
 namespace {
 
+using mi::AttnArgs;
+using mi::kNegBig;
+
 constexpr int D = mi::kHeadDim;
-constexpr float kNegBig = -1e30f;
 constexpr int kColPitch = D + 4;  // f32 per column of the merge buffer
 
 // Waves of a workgroup: two to a SIMD where the accumulators leave room.
 constexpr int waves(int ct) { return ct == 1 ? 8 : 4; }
 // Tiles below which a workgroup is not split further: one to a wave.
 constexpr int kMinTiles = 8;
-
-struct AttnArgs {
-  mi::PagedView pv;
-  const _Float16* q;
-  int64_t q_ts, q_hs;
-  const void* gate;  // f16, or f32 (gate32), or null
-  int64_t g_ts, g_hs;
-  _Float16* out;     // [n][G R][D]
-  float* part_o;     // [2 workgroups][16 CT][D]
-  float* part_ml;    // [2 workgroups][16 CT][2]
-  int2* seg;         // [batch G ncb]: first slot and last workgroup of an item, or -1
-  int32_t n, R, max_q, max_len, wgs, ncb, gate32, dsplit;
-};
 
 // A sequence as its work: ncb blocks of 16 CT columns per KV head, each over
 // ntiles tiles of 32 rows.  Items of a sequence are (KV head, block); its weight,
@@ -62,93 +51,6 @@ __device__ __forceinline__ Seq get_seq(const AttnArgs& a, int s) {
   r.ncb = r.bad ? 0 : (r.nq * a.R + 16 * CT - 1) / (16 * CT);
   r.ntiles = r.bad ? 0 : (r.len + 31) >> 5;
   return r;
-}
-
-// out of four columns: the gate, then f16.
-__device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
-  if (a.gate) {
-    const int64_t gi = tok * a.g_ts + head * a.g_hs + d;
-    f32x4 g;
-    if (a.gate32) {
-      g = *(const f32x4*)((const float*)a.gate + gi);
-    } else {
-      const f16x4 h = *(const f16x4*)((const _Float16*)a.gate + gi);
-      g = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) x[e] = mi::gate_mul(x[e], g[e]);
-  }
-  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * D + d) =
-      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-}
-
-// Sum over the workgroup and the exclusive prefix of each thread's x.
-template <int NT>
-__device__ __forceinline__ int block_scan(int x, int& before, int* lds) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int run = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(run, d, 64);
-    if (lane >= d) run += y;
-  }
-  __syncthreads();  // lds may hold an earlier scan's
-  if (lane == 63) lds[w] = run;
-  __syncthreads();
-  int base = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 64; i++) {
-    if (i < w) base += lds[i];
-    total += lds[i];
-  }
-  before = base + run - x;
-  return __builtin_amdgcn_readfirstlane(total);
-}
-
-// The sequence s that holds weight unit `unit(total weight)` of weight(s), and the
-// weight before it; s = 0 where no sequence does.  (The host holds the tiles of a
-// batch, over KV heads and blocks, below 2^31.)
-template <int NT, typename W, typename F>
-__device__ __forceinline__ void find_seq(int batch, W weight, F unit, int& s, int& before) {
-  __shared__ int lds[NT / 64 + 2];
-  const int t = threadIdx.x;
-  s = 0;
-  before = 0;
-  if (batch == 1) {
-    unit(__builtin_amdgcn_readfirstlane(weight(0)));
-    return;
-  }
-  int total = 0, pre = 0, x = 0;
-  for (int c = 0; c < batch; c += NT) {
-    x = c + t < batch ? weight(c + t) : 0;
-    total += block_scan<NT>(x, pre, lds);
-  }
-  const int want = unit(total);
-  if (want >= total) return;
-  int base = 0;
-  for (int c = 0; c < batch; c += NT) {
-    if (batch > NT) {  // one pass of a small batch has them already
-      x = c + t < batch ? weight(c + t) : 0;
-      const int sum = block_scan<NT>(x, pre, lds);
-      if (want >= base + sum) {  // uniform
-        base += sum;
-        continue;
-      }
-    }
-    if (base + pre <= want && want < base + pre + x) {
-      lds[NT / 64] = c + t;
-      lds[NT / 64 + 1] = base + pre;
-    }
-    break;
-  }
-  __syncthreads();
-  s = __builtin_amdgcn_readfirstlane(lds[NT / 64]);
-  before = __builtin_amdgcn_readfirstlane(lds[NT / 64 + 1]);
-}
-
-// Eight columns of Q in dequant_row's order.
-__device__ __forceinline__ f16x8 in_order(f16x8 x) {
-  return f16x8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
 }
 
 // One wave's state over the tiles of an item.
@@ -357,7 +259,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
   const int G = a.pv.G;
   bool chunks = true;
   auto parts = [](int ntiles) { return (ntiles + kMinTiles - 1) / kMinTiles; };
-  find_seq<NT>(
+  mi::find_seq<NT>(
       a.pv.batch,
       [&](int i) {
         const Seq q = get_seq<CT, false>(a, i);
@@ -371,7 +273,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       },
       s, before);
   if (!chunks)
-    find_seq<NT>(
+    mi::find_seq<NT>(
         a.pv.batch,
         [&](int i) {
           const Seq q = get_seq<CT, false>(a, i);
@@ -426,7 +328,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
         for (int i = 0; i < 8; i++) {  // group i / 2, step i % 2
           const f16x8 x = *(const f16x8*)(qp + 64 * (i >> 1) + 8 * (i & 1));
           if constexpr (CT == 1) q1[i] = x;
-          else qbuf[(ct * 8 + i) * 64 + lane] = in_order(x);
+          else qbuf[(ct * 8 + i) * 64 + lane] = mi::in_order(x);
         }
       }
     }
@@ -460,7 +362,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       if constexpr (CT == 1) {  // behind the tile's loads: it waits for Q's
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < 8; i++) q1[i] = in_order(q1[i]);
+        for (int i = 0; i < 8; i++) q1[i] = mi::in_order(q1[i]);
       }
       const uint8_t* next = base(id1, t + NW);
       for (; t < tm; t += NW) {
@@ -526,7 +428,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
         if (whole) {
           const int tok = col / a.R;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, x * inv);
+          mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, x * inv);
         } else {
           *(f32x4*)(a.part_o + (col0 + 16 * ct + c) * D + d) = x;
           if (d == 0) *(float2*)(a.part_ml + (col0 + 16 * ct + c) * 2) = float2{tbox[c], sum};
@@ -623,11 +525,14 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
     y += acc[g * d4 + t] * f;
   }
   const int tok = col / a.R;
-  put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y * (total == 0.f ? 0.f : 1.f / total));
+  mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y * (total == 0.f ? 0.f : 1.f / total));
 }
 
 // Column blocks of 16 a workgroup takes: 2 where a sequence has more than one.
 int column_blocks(int32_t max_q, int R) { return (int64_t)max_q * R <= 16 ? 1 : 2; }
+
+// Whether the prompts' form serves a call.
+bool many_columns(int32_t max_q, int R) { return (int64_t)max_q * R > 32; }
 
 struct Plan {
   int ct, ncb, wgs, dsplit;
@@ -687,9 +592,12 @@ extern "C" size_t mi_attn_paged_workspace_size(int32_t batch, int32_t n, int32_t
   if (check_heads(num_q_heads, num_kv_heads) != MI_OK || batch <= 0 || n <= 0 || max_q <= 0 ||
       max_len < 0)
     return 0;
-  const Plan p = make_plan(batch, std::min(max_q, n), max_len, num_q_heads, num_kv_heads);
+  max_q = std::min(max_q, n);
+  const Plan p = make_plan(batch, max_q, max_len, num_q_heads, num_kv_heads);
   if (p.tiles >= INT32_MAX) return 0;
-  return p.bytes();
+  return many_columns(max_q, num_q_heads / num_kv_heads)
+             ? mi::paged_prefill_workspace(batch, n, max_q, max_len, num_q_heads, num_kv_heads)
+             : p.bytes();
 }
 
 extern "C" mi_status mi_attn_paged(
@@ -729,9 +637,12 @@ extern "C" mi_status mi_attn_paged(
   if (p.tiles >= INT32_MAX)
     return mi::fail(MI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d rows in one call", batch, max_q,
                     max_len);
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.bytes())
-    return mi::fail(MI_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes,
-                    p.bytes());
+  const bool many = many_columns(max_q, num_q_heads / num_kv_heads);
+  const size_t need = many ? mi::paged_prefill_workspace(batch, n, max_q, max_len, num_q_heads,
+                                                         num_kv_heads)
+                           : p.bytes();
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
+    return mi::fail(MI_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.q = (const _Float16*)q;
   a.q_ts = q_token_stride;
   a.q_hs = q_head_stride;
@@ -751,5 +662,6 @@ extern "C" mi_status mi_attn_paged(
   a.ncb = p.ncb;
   a.dsplit = p.dsplit;
   const hipStream_t s = (hipStream_t)stream;
+  if (many) return mi::paged_prefill(a, workspace, s);
   return p.ct == 1 ? run<1>(a, p, s) : run<2>(a, p, s);
 }

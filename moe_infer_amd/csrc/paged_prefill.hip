@@ -1,0 +1,583 @@
+// Attention over the paged 4-bit cache for many tokens: prompts, and chunks
+// behind cached rows.
+//
+// A workgroup takes 128 rows, the (token, query head of the group) pairs of
+// 128 / R consecutive tokens of one sequence and KV head, and walks the keys
+// that they see in tiles of 64.  The four waves dequantise a tile once into
+// LDS as f16, in MFMA operand order; wave (qb, kp) multiplies rows 64 qb .. + 63
+// with keys 32 kp .. + 31 of it (v_mfma_f32_32x32x16_f16, S^T = K Q^T, O^T += V^T
+// P^T), so that every operand read from LDS feeds two products, and the two
+// key halves join at the end.
+//
+// Bound: the matrix units.  A tile is 64 MFMAs of 32 clocks to a wave, one wave
+// to a SIMD; what else it needs is issued between them: the next tile's
+// dequantisation (16 words a thread) between those of K Q^T, the softmax of tile t
+// between those of P V of tile t - 1.  O^T of 64 rows takes the 256 accumulation
+// registers, so the scores have to come out in ordinary ones: their MFMAs are
+// asm, which the compiler would otherwise give the accumulation form as well.
+//
+// The keys of a block of rows are cut into pieces where one walk would outlast an
+// even share of the call (a few tokens behind a long context): pieces leave
+// partials, paged_prefill_merge_kernel joins them.
+#include <algorithm>
+#include <cmath>
+
+#include "paged_attn.h"
+
+namespace {
+
+using mi::AttnArgs;
+using mi::kNegBig;
+
+constexpr int D = mi::kHeadDim;
+constexpr int kRows = 128;   // rows of a workgroup
+constexpr int kKeys = 64;    // keys of a tile
+constexpr int kHalf = 16384;  // bytes of 32 keys, K or V, as f16
+constexpr int kShare = 256;  // even shares of a call: one per CU
+constexpr int kMinPiece = 8;  // tiles below which keys are not cut further
+constexpr int kSplitBlocks = 256, kSlots = 512;  // most blocks that are cut, and pieces of them
+
+struct PrefillExtra {
+  float* part_o;    // [kSlots][kRows][D]
+  float* part_ml;   // [kSlots][kRows][2]
+  int4* blocks;     // [kSplitBlocks]: sequence, KV head, block, index of its second piece
+  int2* count;      // blocks that are cut, tiles of a piece
+};
+
+// A sequence as blocks of tb tokens.
+struct Blocks {
+  int q0, nq, len, nb, tb;
+  bool bad;
+  __device__ __forceinline__ int first() const { return len - nq; }
+  // rows that block b's last token sees, and tiles of them
+  __device__ __forceinline__ int end(int b) const { return first() + min(nq, tb * (b + 1)); }
+  __device__ __forceinline__ int tiles(int b) const { return max(end(b) + kKeys - 1, 0) / kKeys; }
+  // First block with more than x tiles; nb where none has.
+  __device__ __forceinline__ int past(int64_t x) const {
+    if (nb == 0 || len <= x * kKeys) return nb;
+    const int64_t y = x * kKeys - first();
+    return y <= 0 ? 0 : (int)((uint32_t)y / (uint32_t)tb);
+  }
+};
+__device__ __forceinline__ Blocks get_blocks(const AttnArgs& a, int s) {
+  Blocks r;
+  a.pv.tokens(s, r.q0, r.nq);
+  r.len = a.pv.kv_len[s];
+  r.bad = r.len < 0 || r.len > a.max_len || r.nq > a.max_q;
+  if (r.nq <= 0 || r.q0 < 0 || (int64_t)r.q0 + r.nq > a.n) r.nq = 0;
+  r.tb = kRows / a.R;
+  r.nb = r.bad ? 0 : (r.nq + r.tb - 1) / r.tb;
+  return r;
+}
+// Pieces of a sequence's blocks (one KV head), each of at most `piece` tiles:
+// piece k of block b exists where b >= past(k piece), piece 0 always.  Those of
+// k >= 1 alone with `more`.
+__device__ __forceinline__ int pieces(const Blocks& q, int piece, bool more) {
+  int n = more ? 0 : q.nb;
+  if (q.nb == 0) return 0;
+  const int most = q.tiles(q.nb - 1);
+  for (int64_t x = piece; x < most; x += piece) n += q.nb - q.past(x);
+  return n;
+}
+
+template <int NT>
+__device__ __forceinline__ double block_sum(double x, double* lds) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) sum += lds[i];
+  return sum;
+}
+
+// Tiles of a piece: an even share of the call's tiles (at least, so that no more
+// than kShare pieces come on top of one per block), or kMinPiece.
+__device__ __forceinline__ int piece_tiles(const AttnArgs& a, double* lds) {
+  double mine = 0.0;
+  for (int s = threadIdx.x; s < a.pv.batch; s += 256) {
+    const Blocks q = get_blocks(a, s);
+    if (q.nb) mine += (double)q.nb * (0.5 * (q.tiles(0) + q.tiles(q.nb - 1)) + 1.0);
+  }
+  const double all = block_sum<256>(mine, lds) * a.pv.G;
+  return __builtin_amdgcn_readfirstlane(max(kMinPiece, (int)ceil(all / kShare)));
+}
+
+__device__ __forceinline__ void mfma_s(f32x16& c, f16x8 a, f16x8 b) {
+  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void mfma_s0(f32x16& c, f16x8 a, f16x8 b) {
+  asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+}
+
+__global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a, const PrefillExtra x) {
+  extern __shared__ char lds[];  // K, V [2][2 halves], their scales; then the join of the key halves
+  __shared__ double sums[4];
+  __shared__ int odd_row[4];  // least masked row whose V group is not finite
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hl = lane >> 5;
+  const int qb = w & 1, kp = w >> 1;
+  const int bid = blockIdx.y * gridDim.x + blockIdx.x;
+  const int G = a.pv.G;
+
+  // ---- which block of which sequence, and which of its tiles
+  const int piece = piece_tiles(a, sums);
+  int s, before, local = -1;
+  mi::find_seq<256>(
+      a.pv.batch, [&](int i) { return pieces(get_blocks(a, i), piece, false); },
+      [&](int total) {
+        local = (uint32_t)bid < (uint32_t)total * (uint32_t)G ? bid : -1;
+        return local < 0 ? total : (int)((uint32_t)bid / (uint32_t)G);
+      },
+      s, before);
+  if (bid == 0) {  // for the merge
+    double cut = 0.0;
+    for (int i = tid; i < a.pv.batch; i += 256) {
+      const Blocks q = get_blocks(a, i);
+      cut += q.nb - q.past(piece);
+    }
+    cut = block_sum<256>(cut, sums);
+    if (tid == 0) *x.count = int2{(int)cut * G, piece};
+  }
+  if (local < 0) return;
+  Blocks q = get_blocks(a, s);
+  q.q0 = __builtin_amdgcn_readfirstlane(q.q0);
+  q.nq = __builtin_amdgcn_readfirstlane(q.nq);
+  q.len = __builtin_amdgcn_readfirstlane(q.len);
+  q.nb = __builtin_amdgcn_readfirstlane(q.nb);
+  const int per = __builtin_amdgcn_readfirstlane(pieces(q, piece, false));
+  local -= G * before;
+  const int h = (int)((uint32_t)local / (uint32_t)per);
+  local -= h * per;
+  int k = 0, b0 = 0;  // piece k of the blocks from b0 on, the last (longest) first
+  while (local >= q.nb - b0) {
+    local -= q.nb - b0;
+    k++;
+    b0 = __builtin_amdgcn_readfirstlane(q.past((int64_t)k * piece));
+  }
+  const int b = q.nb - 1 - local;
+  const int tok0 = b * q.tb, ntok = min(q.tb, q.nq - tok0), nrows = ntok * a.R;
+  const int nt_all = q.tiles(b), cuts = max(1, (nt_all + piece - 1) / piece);
+  const int first = q.first() + tok0;  // row of the block's first token
+  const int end = first + ntok;
+  const int ta = (int)((int64_t)nt_all * k / cuts), tz = (int)((int64_t)nt_all * (k + 1) / cuts);
+
+  if (tid < 4) odd_row[tid] = INT32_MAX;
+
+  // ---- Q^T operands of the wave's 64 rows, and the rows that they see
+  f16x8 qf[2][16];
+  int lim[2];
+#pragma unroll
+  for (int c = 0; c < 2; c++) {
+    const int r = 64 * qb + 32 * c + col;
+    const int rr = r < nrows ? r : 0, tok = rr / a.R, head = h * a.R + rr - tok * a.R;
+    lim[c] = r < nrows ? first + tok + 1 : 0;
+    const _Float16* qp = a.q + (int64_t)(q.q0 + tok0 + tok) * a.q_ts + head * a.q_hs + 8 * hl;
+#pragma unroll
+    for (int ks = 0; ks < 16; ks++) qf[c][ks] = mi::in_order(*(const f16x8*)(qp + 16 * ks));
+  }
+
+  // ---- a tile's words: those of the 32-row tiles 2 t and 2 t + 1.  A thread takes a
+  // 16-byte piece of K and of V of each, and one word of the scales of one of them,
+  // which go through LDS a tile earlier (in registers every thread would hold 20
+  // words of them).
+  u32x4 rk[2], rv[2];
+  uint32_t sk, sv;
+  bool lost = false;
+  auto base = [&](int t32) -> __amdgpu_buffer_rsrc_t {
+    const uint8_t* p = nullptr;
+    if (t32 * 32 < end) {
+      p = a.pv.tile(s, h, t32);
+      lost = lost || !p;
+    }
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, p ? mi::kTileBytes : 0,
+                                             0x00020000);
+  };
+  const int m16 = lane & 15, quad = lane >> 4;
+  const int su = w >> 1, sat = 4 * (tid & 127);  // the thread's word of scales: tile, offset
+  auto load_k = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      rk[u] = __builtin_amdgcn_raw_buffer_load_b128(base(2 * t + u), 16 * tid, 0, 0);
+  };
+  auto load_v = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+      rv[u] = __builtin_amdgcn_raw_buffer_load_b128(base(2 * t + u), mi::kVCodes + 16 * tid, 0, 0);
+  };
+  auto load_sk = [&](int t) {
+    sk = __builtin_amdgcn_raw_buffer_load_b32(base(2 * t + su), mi::kKScale + sat, 0, 0);
+  };
+  auto load_sv = [&](int t) {
+    sv = __builtin_amdgcn_raw_buffer_load_b32(base(2 * t + su), mi::kVScale + sat, 0, 0);
+  };
+  const uint32_t x16 = mi::sixteens();
+  char* const kbuf = lds;
+  char* const vbuf = lds + 4 * kHalf;
+  char* const ksc = lds + 8 * kHalf;  // [2][2 tiles][512]
+  char* const vsc = ksc + 2048;
+  auto put_sk = [&](int t) { *(uint32_t*)(ksc + (t & 1) * 1024 + 4 * tid) = sk; };
+  // V's word: scale or offset of rows 4 quad + i and 16 more, of group g.  Rows that no
+  // token of the block sees read as zero, and so does what is not finite in rows that
+  // some token does not see (the MFMA would make NaN of 0 * NaN for it); the
+  // tokens that do see such a row get their NaN at the end.
+  auto put_sv = [&](int t) {
+    uint32_t y = sv;
+    if (kKeys * (t + 1) > first + 1) {  // uniform: not seen whole
+      const int i = tid & 3, sq = (tid >> 3) & 3, g = (tid >> 5) & 3;
+      const int row = kKeys * t + 32 * su + 4 * sq + i;
+      y &= (row < end ? 0xffffu : 0u) | (row + 16 < end ? 0xffff0000u : 0u);
+      const uint32_t odd = ((y & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+      if (odd) {
+        atomicMin(&odd_row[g], odd & 0x8000u ? row : row + 16);
+        y &= ~((odd >> 15) * 0xffffu);
+      }
+    }
+    *(uint32_t*)(vsc + (t & 1) * 1024 + 4 * tid) = y;
+  };
+  // The wave's pieces of K: rows 16 (w / 2) + m16, groups 2 (w % 2) and the next.  Word j:
+  // operand 4 (2 (w % 2) + j / 2) + quad, lane half j % 2, and the slot whose score lands
+  // where P wants the key (slot 16 s + 8 (e / 4) + 4 l + e % 4 of lane half l is key
+  // 16 (e % 2) + 4 (2 s + l) + e / 2)
+  const int kslot = 16 * (m16 >> 3) + 8 * ((m16 >> 1) & 1) + 4 * ((m16 >> 2) & 1) + 2 * (m16 & 1) + (w >> 1);
+  const int kdst = ((8 * (w & 1) + quad) * 2 * 32 + kslot) * 16;
+  const int ksrc = 16 * (16 * (w >> 1) + m16) + 8 * (w & 1);
+  // V word j: product quad / 2, block 2 w + j / 2, lane half quad % 2, slot 16 (j % 2) + n
+  const int vdst = (((quad >> 1) * 8 + 2 * w) * 2 * 32 + (quad & 1) * 32 + m16) * 16;
+  const int vsrc = 32 * (4 * w + quad);
+  auto put_k = [&](int t, int u, int j) {
+    const f16x2 so = *(const f16x2*)(ksc + (t & 1) * 1024 + 512 * u + ksrc + 4 * (j >> 1));
+    *(f16x8*)(kbuf + ((t & 1) * 2 + u) * kHalf + kdst + (((j >> 1) * 4 * 2 + (j & 1)) * 32) * 16) =
+        mi::dequant_row(rk[u][j], f16x2{so[0], so[0]}, f16x2{so[1], so[1]}, x16);
+  };
+  f16x8 vs, vo;
+  auto put_v = [&](int t, int u, int j) {
+    if (j == 0) {
+      vs = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc);
+      vo = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc + 16);
+    }
+    *(f16x8*)(vbuf + ((t & 1) * 2 + u) * kHalf + vdst + ((j >> 1) * 64 + 16 * (j & 1)) * 16) =
+        mi::dequant_col(rv[u][j], vs, vo, x16);
+  };
+
+  constexpr float c2 = mi::kLog2e / 16.f;  // softmax scale 1 / sqrt(256), in base 2
+  f32x16 acc[2][8];
+  float m[2] = {kNegBig, kNegBig}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < 2; c++)
+#pragma unroll
+    for (int i = 0; i < 8; i++) acc[c][i] = f32x16{};
+  f16x8 p[2][2];
+#pragma unroll
+  for (int c = 0; c < 2; c++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) p[c][i] = f16x8{};
+
+  if (ta < tz) {
+    // the first walk's products with no weights read a buffer of zeros
+    for (int i = tid; i < 2 * kHalf / 16; i += 256)
+      ((u32x4*)(vbuf + ((ta - 1) & 1) * 2 * kHalf))[i] = u32x4{};
+    load_sk(ta);
+    load_k(ta);
+    put_sk(ta);
+    load_sk(ta + 1);
+    load_sv(ta);
+    load_v(ta);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) put_k(ta, u, j);
+    load_k(ta + 1);
+    put_sk(ta + 1);
+    put_sv(ta);
+    load_sk(ta + 2);
+    load_sv(ta + 1);
+  }
+  __syncthreads();
+  for (int t = ta; t < tz; t++) {
+    // K Q^T of tile t; between its products the next tile's K and this tile's V go
+    // to LDS (what lies behind the last tile is read as zeros)
+    f32x16 sc[2];
+    {
+      const char* const kr = kbuf + ((t & 1) * 2 + kp) * kHalf + lane * 16;
+      constexpr int kRing = 4;
+      f16x8 kf[kRing];
+#pragma unroll
+      for (int i = 0; i < kRing; i++) kf[i] = *(const f16x8*)(kr + 1024 * i);
+#pragma unroll
+      for (int ks = 0; ks < 16; ks++) {
+        if (ks == 0) {
+          mfma_s0(sc[0], kf[0], qf[0][0]);
+          mfma_s0(sc[1], kf[0], qf[1][0]);
+        } else {
+          mfma_s(sc[0], kf[ks % kRing], qf[0][ks]);
+          mfma_s(sc[1], kf[ks % kRing], qf[1][ks]);
+        }
+        if (ks + kRing < 16) kf[ks % kRing] = *(const f16x8*)(kr + 1024 * (ks + kRing));
+        if (ks < 8) put_k(t + 1, ks >> 2, ks & 3);
+        else put_v(t, (ks - 8) >> 2, ks & 3);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    put_sk(t + 2);  // its buffer held tile t's, which the last walk read
+    put_sv(t + 1);
+    load_sk(t + 3);
+    load_sv(t + 2);
+    load_v(t + 1);
+    load_k(t + 2);
+    // the products' results are read by ordinary instructions from here on
+    asm volatile("s_nop 15\n\ts_nop 3" : "+v"(sc[0]), "+v"(sc[1]));
+    const int row0 = kKeys * t + 32 * kp;
+    if (row0 + 32 > first + 1) {  // some row of the block does not see some key (uniform)
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+          if (row0 + 16 * (e & 1) + 4 * (2 * (e >> 3) + hl) + ((e & 7) >> 1) >= lim[c])
+            sc[c][e] = -__builtin_inff();
+    }
+    // The reference point moves only when weights would pass 2^8.
+    float shift[2] = {1.f, 1.f};
+    bool moved = false;
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      float top = fmaxf(sc[c][0], sc[c][1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) top = fmaxf(fmaxf(top, sc[c][e]), sc[c][e + 1]);
+      top = mi::max_xor32(top) * c2;
+      if (__any(top > m[c] + 8.f)) {
+        const float mn = fmaxf(m[c], top);
+        shift[c] = __builtin_amdgcn_exp2f(m[c] - mn);
+        m[c] = mn;
+        l[c] *= shift[c];
+        moved = true;
+      }
+    }
+    // V^T P of tile t - 1, with tile t's weights between the products: two scores of
+    // each of the 16 slots
+    f16x8 pn[2][2];
+    {
+      const char* const vr = vbuf + (((t - 1) & 1) * 2 + kp) * kHalf + lane * 16;
+      constexpr int vRing = 4;
+      f16x8 vf[vRing];
+#pragma unroll
+      for (int i = 0; i < vRing; i++) vf[i] = *(const f16x8*)(vr + 1024 * i);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {  // product i / 8, block i % 8; scores 2 i, 2 i + 1
+        const int c = i >> 3, e = 2 * (i & 7);
+        acc[0][i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % vRing], p[0][i >> 3], acc[0][i & 7], 0, 0, 0);
+        const float ya = __builtin_amdgcn_exp2f(fmaf(sc[c][e], c2, -m[c]));
+        __builtin_amdgcn_sched_barrier(0);
+        acc[1][i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % vRing], p[1][i >> 3], acc[1][i & 7], 0, 0, 0);
+        if (i + vRing < 16) vf[i % vRing] = *(const f16x8*)(vr + 1024 * (i + vRing));
+        const float yb = __builtin_amdgcn_exp2f(fmaf(sc[c][e + 1], c2, -m[c]));
+        l[c] += ya + yb;
+        pn[c][e >> 3][e & 7] = (_Float16)ya;  // the MFMA's operand: off by 2^-11 of itself at most
+        pn[c][e >> 3][(e & 7) + 1] = (_Float16)yb;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (moved) {  // uniform
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          // sixteen at a time, in ordinary registers and back: all would not fit
+          asm volatile("" : "+a"(acc[c][i]));
+          acc[c][i] *= shift[c];
+          asm volatile("" : "+a"(acc[c][i]));
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+      for (int i = 0; i < 2; i++) p[c][i] = pn[c][i];
+    mi::sync_lds();
+  }
+  if (ta < tz) {
+    const char* const vr = vbuf + (((tz - 1) & 1) * 2 + kp) * kHalf + lane * 16;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const f16x8 vf = *(const f16x8*)(vr + 1024 * i);
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+        acc[c][i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[c][i >> 3], acc[c][i & 7], 0, 0, 0);
+    }
+  }
+
+  // ---- the key halves join: wave (qb, kp) finishes rows 32 kp of its 64 and hands
+  // the others to its partner.  The waves of the upper half swap their blocks first,
+  // so that every register index is a constant.
+#pragma unroll
+  for (int c = 0; c < 2; c++) {
+    l[c] = mi::sum_xor32(l[c]);
+    if (lost) l[c] = __builtin_nanf("");
+  }
+  __syncthreads();  // every wave is done with the tiles
+  if (kp) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const f32x16 y = acc[0][i];
+      acc[0][i] = acc[1][i];
+      acc[1][i] = y;
+    }
+    const float tm = m[0], tl = l[0];
+    m[0] = m[1];
+    l[0] = l[1];
+    m[1] = tm;
+    l[1] = tl;
+    lim[0] = lim[1];
+  }
+  f32x4* const box = (f32x4*)lds;                    // [2 qb][2 kp][32][64]
+  float2* const mlbox = (float2*)(box + 4 * 32 * 64);  // [2][2][32]
+  {
+    f32x4* const dst = box + (2 * qb + 1 - kp) * 32 * 64;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; e4++)
+        dst[(i * 4 + e4) * 64 + lane] = f32x4{acc[1][i][4 * e4], acc[1][i][4 * e4 + 1],
+                                              acc[1][i][4 * e4 + 2], acc[1][i][4 * e4 + 3]};
+    if (hl == 0) mlbox[(2 * qb + 1 - kp) * 32 + col] = float2{m[1], l[1]};
+  }
+  mi::sync_lds();
+  const f32x4* const src = box + (2 * qb + kp) * 32 * 64;
+  const float2 ml = mlbox[(2 * qb + kp) * 32 + col];
+  const float top = fmaxf(m[0], ml.x);
+  float fa = __builtin_amdgcn_exp2f(m[0] - top), fb = __builtin_amdgcn_exp2f(ml.x - top);
+  const float sum = l[0] * fa + ml.y * fb;
+  const int r = 64 * qb + 32 * kp + col;
+  if (cuts == 1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    fa *= inv;
+    fb *= inv;
+  }
+  int64_t slot = 0;
+  if (cuts > 1) {  // slots: the first pieces of the blocks that are cut, then the others
+    double cut = 0.0, more = 0.0;
+    for (int i = tid; i < s; i += 256) {
+      const Blocks o = get_blocks(a, i);
+      cut += o.nb - o.past(piece);
+      more += pieces(o, piece, true);
+    }
+    const int cut0 = (int)block_sum<256>(cut, sums), more0 = (int)block_sum<256>(more, sums);
+    const int b1 = q.past(piece), mine = q.nb - b1;
+    const int at = cut0 * G + h * mine + (q.nb - 1 - b);                 // of the blocks
+    const int second = more0 * G + h * (per - q.nb) + (q.nb - 1 - b);    // of the pieces k >= 1
+    if (k == 0) {
+      slot = at;
+      if (tid == 0 && at < kSplitBlocks) x.blocks[at] = int4{s, h, b, second};
+    } else {
+      int add = 0;
+      for (int kk = 1; kk < k; kk++) add += q.nb - q.past((int64_t)kk * piece);
+      slot = kSplitBlocks + second + add;
+    }
+    if (slot >= kSlots || (k == 0 && slot >= kSplitBlocks)) return;  // cannot be: piece_tiles
+    if (hl == 0 && r < nrows)
+      ((float2*)x.part_ml)[slot * kRows + r] = float2{top, sum};
+  }
+  if (r >= nrows) return;
+  const int tok = r / a.R, head = h * a.R + r - tok * a.R;
+#pragma unroll
+  for (int g = 0; g < 4; g++) {
+    const bool odd = odd_row[g] < lim[0];
+#pragma unroll
+    for (int nh = 0; nh < 2; nh++) {
+      // value (n, j) of columns 64 g + 32 nh + 16 hl + 4 n + j: block 2 g + j / 2, element
+      // 8 (j % 2) + 4 nh + n
+      f32x4 y[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int i = 2 * g + (j >> 1), e4 = 2 * (j & 1) + nh;
+        const f32x4 o = src[(i * 4 + e4) * 64 + lane];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          float v = acc[0][i][4 * e4 + n] * fa + o[n] * fb;
+          if (odd) v = __builtin_nanf("");
+          y[n][j] = v;
+        }
+      }
+      const int d = 64 * g + 32 * nh + 16 * hl;
+#pragma unroll
+      for (int n = 0; n < 4; n++) {
+        if (cuts == 1) mi::put4(a, q.q0 + tok0 + tok, head, d + 4 * n, y[n]);
+        else *(f32x4*)(x.part_o + (slot * kRows + r) * D + d + 4 * n) = y[n];
+      }
+    }
+  }
+}
+
+// Joins the pieces of the blocks that are cut: a workgroup per (block, 16 rows), a
+// wave per row and four columns a thread.  A workgroup per sequence behind them
+// makes every token NaN of one beyond max_q or max_len.
+__global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const AttnArgs a, const PrefillExtra x) {
+  if (blockIdx.x >= 8 * kSplitBlocks) {
+    const Blocks q = get_blocks(a, blockIdx.x - 8 * kSplitBlocks);
+    const int width = a.pv.G * a.R * D;
+    for (int tok = 0; tok < (q.bad ? q.nq : 0); tok++)
+      for (int i = threadIdx.x; i < width; i += 256)
+        a.out[(int64_t)(q.q0 + tok) * width + i] = (_Float16)__builtin_nanf("");
+    return;
+  }
+  const int at = blockIdx.x >> 3, part = blockIdx.x & 7;
+  const int2 c = *x.count;
+  if (at >= min(c.x, kSplitBlocks)) return;
+  const int4 blk = x.blocks[at];
+  const int s = blk.x, h = blk.y, b = blk.z, second = blk.w, piece = c.y;
+  const Blocks q = get_blocks(a, s);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int nrows = min(q.tb, q.nq - b * q.tb) * a.R, cuts = (q.tiles(b) + piece - 1) / piece;
+  for (int r = 16 * part + w; r < min(16 * part + 16, nrows); r += 4) {
+    float top = kNegBig, sum = 0.f;
+    f32x4 y = {};
+    int add = 0;
+    for (int k = 0; k < cuts; k++) {
+      const int64_t slot = k ? kSplitBlocks + second + add : at;
+      if (k) add += q.nb - q.past((int64_t)k * piece);
+      const float2 ml = ((const float2*)x.part_ml)[slot * kRows + r];
+      const f32x4 o = *(const f32x4*)(x.part_o + (slot * kRows + r) * D + 4 * lane);
+      const float mn = fmaxf(top, ml.x), f = __builtin_amdgcn_exp2f(top - mn),
+                  g = __builtin_amdgcn_exp2f(ml.x - mn);
+      sum = sum * f + ml.y * g;
+      y = y * f + o * g;
+      top = mn;
+    }
+    const int tok = r / a.R;
+    mi::put4(a, q.q0 + b * q.tb + tok, h * a.R + r - tok * a.R, 4 * lane,
+             y * (sum == 0.f ? 0.f : 1.f / sum));
+  }
+}
+
+constexpr int kLds = 8 * kHalf + 2 * 2048;
+
+}  // namespace
+
+namespace mi {
+
+size_t paged_prefill_workspace(int32_t, int32_t, int32_t, int32_t, int, int) {
+  return (size_t)kSlots * kRows * (D + 2) * sizeof(float) + kSplitBlocks * sizeof(int4) + 64;
+}
+
+mi_status paged_prefill(AttnArgs& a, void* workspace, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  MI_TRY(set_lds_limit((const void*)paged_prefill_kernel, kLds, done));
+  PrefillExtra x;
+  x.part_o = (float*)workspace;
+  x.part_ml = x.part_o + (size_t)kSlots * kRows * D;
+  x.blocks = (int4*)(x.part_ml + (size_t)kSlots * kRows * 2);
+  x.count = (int2*)(x.blocks + kSplitBlocks);
+  const int tb = kRows / a.R;
+  // blocks of the batch's sequences, and the pieces that come on top
+  const int64_t wgs = ((int64_t)a.n / tb + a.pv.batch) * a.pv.G + kShare;
+  const int64_t gx = std::min<int64_t>(wgs, 1 << 22);
+  MI_HIP(launch("paged_prefill", paged_prefill_kernel,
+                dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)), dim3(256), kLds, s, a, x));
+  MI_HIP(launch("paged_merge", paged_prefill_merge_kernel, dim3((unsigned)(8 * kSplitBlocks + a.pv.batch)),
+                dim3(256), 0, s, a, x));
+  return MI_OK;
+}
+
+}  // namespace mi
