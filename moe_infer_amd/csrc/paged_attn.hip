@@ -16,6 +16,7 @@
 // partials that paged_merge_kernel joins.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "paged_attn.h"
 
@@ -27,8 +28,10 @@ using mi::kNegBig;
 constexpr int D = mi::kHeadDim;
 constexpr int kColPitch = D + 4;  // f32 per column of the merge buffer
 
-// Waves of a workgroup: two to a SIMD where the accumulators leave room.
+// Waves of a workgroup, and the tiles that each has under way: two waves to a SIMD where
+// the accumulators leave room, else two tiles.
 constexpr int waves(int ct) { return ct == 1 ? 8 : 4; }
+constexpr int ahead(int ct) { return ct == 1 ? 1 : 2; }
 // Tiles below which a workgroup is not split further: one to a wave.
 constexpr int kMinTiles = 8;
 
@@ -53,25 +56,12 @@ __device__ __forceinline__ Seq get_seq(const AttnArgs& a, int s) {
   return r;
 }
 
-// One wave's state over the tiles of an item.
-template <int CT>
-struct Wave {
-  f32x4 o[CT][16];
-  float m[CT], l[CT];
+// A tile in registers, on its way from memory: the words and scales that a lane's
+// operands are made of.  (Scales by way of LDS, a sixteenth of the registers, cost
+// a decode step 5 %: their reads wait where these are there.)
+struct Tile {
   u32x4 k[4], v[4];
   f16x8 ks[2], vs[4], vo[4];
-  int lim[CT];  // rows that the lane's columns see
-  uint32_t x16;
-
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      m[ct] = kNegBig;
-      l[ct] = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; i++) o[ct][i] = f32x4{};
-    }
-  }
   // A tile as a buffer of its size, or of none: then the loads below return zeros
   // and move nothing, so the last tile of a wave prefetches without a branch
   // (whose two ways would need the loaded registers copied, and waited for).
@@ -98,16 +88,36 @@ struct Wave {
       vo[i] = __builtin_bit_cast(f16x8, load(b, 32 * (lane >> 4), mi::kVScale + 128 * i + 16));
     }
   }
+};
 
-  // One tile, rows row0 .. row0 + 31; `next` (or null) is loaded on the way.
-  // MASKED: some column does not see some row; lim1: rows that some column sees.
-  template <bool MASKED, typename Q>
-  __device__ __forceinline__ void tile(__amdgpu_buffer_rsrc_t next, int row0, int lim1, int lane, Q q) {
+// One wave's state over the tiles of an item.
+template <int CT>
+struct Wave {
+  f32x4 o[CT][16];
+  float m[CT], l[CT];
+  f16x8 q[CT][8];  // Q^T operands, group f / 2, step f % 2
+  int lim[CT];     // rows that the lane's columns see
+  uint32_t x16;
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      m[ct] = kNegBig;
+      l[ct] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[ct][i] = f32x4{};
+    }
+  }
+
+  // One tile, rows row0 .. row0 + 31; `next` is loaded in its place on the way.
+  // MASKED: some column may not see some row; lim1: rows that some column sees.
+  template <bool MASKED>
+  __device__ __forceinline__ void tile(Tile& b, __amdgpu_buffer_rsrc_t next, int row0, int lim1, int lane) {
     const int quad = lane >> 4;
     // the words as they are here: without this, their shifts move up to the loads,
     // three registers more for each
 #pragma unroll
-    for (int i = 0; i < 4; i++) asm volatile("" : "+v"(k[i]));
+    for (int i = 0; i < 4; i++) asm volatile("" : "+v"(b.k[i]));
     f32x4 sc[CT][2];
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) sc[ct][0] = sc[ct][1] = f32x4{};
@@ -117,25 +127,22 @@ struct Wave {
       f16x8 ka[2];
 #pragma unroll
       for (int sub = 0; sub < 2; sub++)
-        ka[sub] = mi::dequant_row(k[2 * sub + (g >> 1)][2 * (g & 1) + step],
-                                  f16x2{ks[sub][2 * g], ks[sub][2 * g]},
-                                  f16x2{ks[sub][2 * g + 1], ks[sub][2 * g + 1]}, x16);
+        ka[sub] = mi::dequant_row(b.k[2 * sub + (g >> 1)][2 * (g & 1) + step],
+                                  f16x2{b.ks[sub][2 * g], b.ks[sub][2 * g]},
+                                  f16x2{b.ks[sub][2 * g + 1], b.ks[sub][2 * g + 1]}, x16);
 #pragma unroll
       for (int ct = 0; ct < CT; ct++) {
-        const f16x8 qf = q(ct, f);
 #pragma unroll
         for (int sub = 0; sub < 2; sub++)
-          sc[ct][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[sub], qf, sc[ct][sub], 0, 0, 0);
+          sc[ct][sub] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[sub], q[ct][f], sc[ct][sub], 0, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);  // a few operands at a time
     }
-    load_k(next, lane);
-    uint32_t poison[CT] = {};  // groups whose values a column must take for not a number
+    b.load_k(next, lane);
+    __builtin_amdgcn_sched_barrier(0);
+    uint32_t in1[4] = {};
     if constexpr (MASKED) {
-      // Keys out of sight weigh nothing whatever they hold: their scores are
-      // replaced, and V, whose MFMA would make NaN of 0 * NaN, is cleared where
-      // no column sees the row or where it is not finite; columns that do see
-      // such a row get their NaN below.
+      // Keys out of sight weigh nothing whatever they hold: their scores are replaced
 #pragma unroll
       for (int ct = 0; ct < CT; ct++)
 #pragma unroll
@@ -143,44 +150,8 @@ struct Wave {
 #pragma unroll
           for (int i = 0; i < 4; i++)
             if (row0 + 16 * sub + 4 * quad + i >= lim[ct]) sc[ct][sub][i] = -__builtin_inff();
-      // in pairs of rows (4 quad + i, 16 more), as the scales lie
-      auto seen = [&](int i, int end) {
-        const int r = row0 + 4 * quad + i;
-        return (r < end ? 0xffffu : 0u) | (r + 16 < end ? 0xffff0000u : 0u);
-      };
-      uint32_t odd = 0;  // halves whose exponent is all ones carry into bit 15
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        u32x4 ws = __builtin_bit_cast(u32x4, vs[g]), wo = __builtin_bit_cast(u32x4, vo[g]);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          ws[i] &= seen(i, lim1);
-          wo[i] &= seen(i, lim1);
-          odd |= ((ws[i] & 0x7c007c00u) + 0x04000400u) | ((wo[i] & 0x7c007c00u) + 0x04000400u);
-        }
-        vs[g] = __builtin_bit_cast(f16x8, ws);
-        vo[g] = __builtin_bit_cast(f16x8, wo);
-      }
-      if (__any((odd & 0x80008000u) != 0)) {
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-          u32x4 ws = __builtin_bit_cast(u32x4, vs[g]), wo = __builtin_bit_cast(u32x4, vo[g]);
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const uint32_t top =
-                (((ws[i] & 0x7c007c00u) + 0x04000400u) | ((wo[i] & 0x7c007c00u) + 0x04000400u)) &
-                0x80008000u;
-            const uint32_t halves = (top >> 15) * 0xffffu;
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++)
-              if (halves & seen(i, lim[ct])) poison[ct] |= 1u << g;
-            ws[i] &= ~halves;
-            wo[i] &= ~halves;
-          }
-          vs[g] = __builtin_bit_cast(f16x8, ws);
-          vo[g] = __builtin_bit_cast(f16x8, wo);
-        }
-      }
+      for (int i = 0; i < 4; i++) in1[i] = seen(row0 + 4 * quad + i, lim1);
     }
     constexpr float c2 = mi::kLog2e / 16.f;  // softmax scale 1 / sqrt(256), in base 2
     f16x8 p[CT];
@@ -199,7 +170,12 @@ struct Wave {
         const float mn = fmaxf(m[ct], top), f = __builtin_amdgcn_exp2f(m[ct] - mn);
         l[ct] *= f;
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[ct][i] *= f;
+        for (int i = 0; i < 16; i++) {
+          // four at a time, in ordinary registers and back: all would not fit
+          if constexpr (CT > 1) asm volatile("" : "+a"(o[ct][i]));
+          o[ct][i] *= f;
+          if constexpr (CT > 1) asm volatile("" : "+a"(o[ct][i]));
+        }
         m[ct] = mn;
       }
 #pragma unroll
@@ -211,28 +187,66 @@ struct Wave {
     }
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-      asm volatile("" : "+v"(v[g]));
+      f16x8 vs = b.vs[g], vo = b.vo[g];
+      bool odd_group = false;
+      uint32_t poison = 0;  // columns that see a value of this group that is not finite
+      if constexpr (MASKED) {
+        // V is cleared where no column sees the row or where it is not finite (its MFMA
+        // would make NaN of 0 * NaN); columns that do see such a row get their NaN
+        // here.  In pairs of rows (4 quad + i, 16 more), as the scales lie; a half
+        // whose exponent is all ones carries into its top bit.
+        u32x4 ws = __builtin_bit_cast(u32x4, vs), wo = __builtin_bit_cast(u32x4, vo);
+        uint32_t odd = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          ws[i] &= in1[i];
+          wo[i] &= in1[i];
+          odd |= ((ws[i] & 0x7c007c00u) + 0x04000400u) | ((wo[i] & 0x7c007c00u) + 0x04000400u);
+        }
+        odd_group = __any((odd & 0x80008000u) != 0);
+        if (odd_group) {
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t top = (((ws[i] & 0x7c007c00u) + 0x04000400u) |
+                                  ((wo[i] & 0x7c007c00u) + 0x04000400u)) &
+                                 0x80008000u;
+            const uint32_t halves = (top >> 15) * 0xffffu;
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++)
+              if (halves & seen(row0 + 4 * quad + i, lim[ct])) poison |= 1u << ct;
+            ws[i] &= ~halves;
+            wo[i] &= ~halves;
+          }
+        }
+        vs = __builtin_bit_cast(f16x8, ws);
+        vo = __builtin_bit_cast(f16x8, wo);
+      }
+      asm volatile("" : "+v"(b.v[g]));
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const f16x8 va = mi::dequant_col(v[g][j], vs[g], vo[g], x16);
+        const f16x8 va = mi::dequant_col(b.v[g][j], vs, vo, x16);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++)
           o[ct][4 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, p[ct], o[ct][4 * g + j], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);  // not all sixteen operands at once
-    }
-    load_v(next, lane);
-    if constexpr (MASKED) {
-#pragma unroll
-      for (int ct = 0; ct < CT; ct++)
-        if (__any(poison[ct] != 0)) {
-          uint32_t all = poison[ct] | __shfl_xor(poison[ct], 16, 64);
+      if constexpr (MASKED)
+        if (odd_group) {
+          uint32_t all = poison | __shfl_xor(poison, 16, 64);
           all |= __shfl_xor(all, 32, 64);
 #pragma unroll
-          for (int i = 0; i < 16; i++)
-            if (all >> (i >> 2) & 1) o[ct][i] += __builtin_nanf("");
+          for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+              o[ct][4 * g + j] += all >> ct & 1 ? __builtin_nanf("") : 0.f;
         }
+      __builtin_amdgcn_sched_barrier(0);  // not all sixteen operands at once
     }
+    b.load_v(next, lane);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // Halves of a pair of rows (r, r + 16) that lie before `end`.
+  static __device__ __forceinline__ uint32_t seen(int r, int end) {
+    return (r < end ? 0xffffu : 0u) | (r + 16 < end ? 0xffff0000u : 0u);
   }
 };
 
@@ -240,13 +254,12 @@ template <int CT>
 __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_kernel(const AttnArgs a) {
   constexpr int NW = waves(CT), NT = 64 * NW;
   extern __shared__ float lds[];
-  // maxima [wave][16 CT], sums [wave][16], largest maxima [16]; for CT > 1 the Q
-  // operands [CT][8][64] of 16 bytes; merge buffer [wave][min(16, columns)][kColPitch]
+  // maxima [wave][16 CT], sums [wave][16], largest maxima [16]; merge buffer
+  // [wave][min(16, columns)][kColPitch]
   float* const mbox = lds;
   float* const lbox = mbox + NW * 16 * CT;
   float* const tbox = lbox + NW * 16;
-  f16x8* const qbuf = (f16x8*)(tbox + 16);
-  float* const mbuf = (float*)(qbuf + (CT > 1 ? CT * 8 * 64 : 0));
+  float* const mbuf = tbox + 16;
   const int mcols = min(16, a.max_q * a.R);
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -315,7 +328,6 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
 
     // the lane's columns: their rows of Q, and the rows they see (columns past the
     // last take the first's, which nothing reads)
-    f16x8 q1[8];  // CT == 1: the Q operands
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
       const int c = c0 + 16 * ct + (lane & 15);
@@ -323,57 +335,57 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       const int tok = in ? c / a.R : 0, head = h * a.R + (in ? c - tok * a.R : 0);
       st.lim[ct] = in ? first + tok + 1 : 0;
       const _Float16* qp = a.q + (sq.q0 + tok) * a.q_ts + head * a.q_hs + 16 * (lane >> 4);
-      if (CT == 1 || w == ct % NW) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {  // group i / 2, step i % 2
-          const f16x8 x = *(const f16x8*)(qp + 64 * (i >> 1) + 8 * (i & 1));
-          if constexpr (CT == 1) q1[i] = x;
-          else qbuf[(ct * 8 + i) * 64 + lane] = mi::in_order(x);
-        }
-      }
+      for (int i = 0; i < 8; i++) st.q[ct][i] = *(const f16x8*)(qp + 64 * (i >> 1) + 8 * (i & 1));
     }
-    if constexpr (CT > 1) __syncthreads();
-    auto q = [&](int ct, int i) {
-      if constexpr (CT == 1) return q1[i];
-      else return qbuf[(ct * 8 + i) * 64 + lane];
-    };
     const int lim0 = first + c0 / a.R + 1;                                       // first column's
     const int lim1 = first + min(sq.nq - 1, (c0 + 16 * CT - 1) / a.R) + 1;       // last column's
     // tiles [t0, tm) are seen whole, [tm, t1) not
     const int tm = max(t0, min(t1, lim0 >> 5));
 
     st.clear();
-    // A page that is not there is read as no bytes and the sums become not a
-    // number.  Pages are looked up two tiles ahead, loads issued one ahead.
+    // A page that is not there is read as no bytes and the sums become not a number.
+    // kAhead tiles are under way, in turn; pages are looked up another one ahead.
+    constexpr int kAhead = ahead(CT);
     bool lost = false;
-    auto base = [&](int32_t id, int t) -> const uint8_t* {
-      if (t >= t1) return nullptr;
-      const uint8_t* p = a.pv.at(id, h, t);
-      lost = lost || !p;
-      return p;
+    auto buffer = [&](int32_t id, int t) {
+      const uint8_t* p = t < t1 ? a.pv.at(id, h, t) : nullptr;
+      lost = lost || (t < t1 && !p);
+      return Tile::buffer(p);
     };
     auto page = [&](int t) { return t < t1 ? a.pv.page(s, t) : -1; };
     int t = t0 + w;
     if (t < t1) {
-      const int32_t id0 = page(t), id1 = page(t + NW);
-      const auto cur = st.buffer(base(id0, t));
-      st.load_k(cur, lane);
-      st.load_v(cur, lane);
-      if constexpr (CT == 1) {  // behind the tile's loads: it waits for Q's
-        __builtin_amdgcn_sched_barrier(0);
+      Tile tiles[kAhead];
+      int32_t id[kAhead + 1];
 #pragma unroll
-        for (int i = 0; i < 8; i++) q1[i] = mi::in_order(q1[i]);
+      for (int i = 0; i <= kAhead; i++) id[i] = page(t + i * NW);
+#pragma unroll
+      for (int i = 0; i < kAhead; i++) {
+        const auto b = buffer(id[i], t + i * NW);
+        tiles[i].load_k(b, lane);
+        tiles[i].load_v(b, lane);
       }
-      const uint8_t* next = base(id1, t + NW);
-      for (; t < tm; t += NW) {
-        const int32_t id = page(t + 2 * NW);
-        st.template tile<false>(st.buffer(next), 32 * t, lim1, lane, q);
-        next = base(id, t + 2 * NW);
+      __builtin_amdgcn_sched_barrier(0);  // behind the tiles' loads: it waits for Q's
+#pragma unroll
+      for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) st.q[ct][i] = mi::in_order(st.q[ct][i]);
+      int32_t ahead_id = id[kAhead];
+      auto step = [&](Tile& x, auto masked) {
+        const auto next = buffer(ahead_id, t + kAhead * NW);
+        ahead_id = page(t + (kAhead + 1) * NW);
+        st.template tile<decltype(masked)::value>(x, next, 32 * t, lim1, lane);
+        t += NW;
+      };
+      while (t + (kAhead - 1) * NW < tm) {
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) step(tiles[i], std::false_type{});
       }
-      for (; t < t1; t += NW) {
-        const int32_t id = page(t + 2 * NW);
-        st.template tile<true>(st.buffer(next), 32 * t, lim1, lane, q);
-        next = base(id, t + 2 * NW);
+      while (t < t1) {  // what some column may not see
+#pragma unroll
+        for (int i = 0; i < kAhead; i++)
+          if (i == 0 || t < t1) step(tiles[i], std::true_type{});
       }
     }
 
@@ -563,7 +575,7 @@ template <int CT>
 mi_status run(AttnArgs& a, const Plan& p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   constexpr int NW = waves(CT);
-  const int fixed = (NW * 16 * (CT + 1) + 16) * (int)sizeof(float) + (CT > 1 ? CT * 8 * 64 * 16 : 0);
+  const int fixed = (NW * 16 * (CT + 1) + 16) * (int)sizeof(float);
   const int per_col = NW * kColPitch * (int)sizeof(float);
   MI_TRY(mi::set_lds_limit((const void*)paged_attn_kernel<CT>, fixed + 16 * per_col, done));
   MI_HIP(mi::launch("paged_attn", paged_attn_kernel<CT>, dim3((unsigned)p.wgs), dim3(64 * NW),
