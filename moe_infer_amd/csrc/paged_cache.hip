@@ -9,7 +9,7 @@
 //
 // A call whose sequences hold any number of tokens goes by tile: a workgroup
 // takes one tile of one sequence and KV head, quantises the rows that the call
-// brings, eight to a wave, and stores whole words; rows of the tile that are
+// brings, four to a wave, and stores whole words; rows of the tile that are
 // not the call's keep their codes (K by 16-byte pieces of one row, V by merging
 // nibbles; no other workgroup holds the same words).  A call of one token per
 // sequence goes by row: a wave takes K or V of one row.
@@ -45,6 +45,9 @@ mi_status paged_view(void* pages, int64_t num_pages, int32_t page_rows, const in
 namespace {
 
 constexpr int D = mi::kHeadDim;
+// Waves to a tile of the append by tile: the chain of a row is long, so rows go side by
+// side (prompts of 6580 tokens, two KV heads: 4 waves 28.8 us without Q).
+constexpr int kTileWaves = 8;
 
 struct AppendArgs {
   mi::PagedView pv;
@@ -55,6 +58,7 @@ struct AppendArgs {
   double eps;
   int32_t n, H;
   int64_t kv_items;           // workgroups of K and V before those of Q
+  int32_t each;               // heads of Q a wave
   mi::RotaryPlan plan;
 };
 
@@ -69,34 +73,59 @@ struct Quant {
   f16x2 so;        // scale, offset of the lane's group
 };
 
-// Codes of the lane's four columns of a row; a group is 16 lanes.
-__device__ __forceinline__ Quant quantise(const double (&z)[4]) {
-  double lo = fmin(fmin(z[0], z[1]), fmin(z[2], z[3]));
-  double hi = fmax(fmax(z[0], z[1]), fmax(z[2], z[3]));
-  bool fine = true;
-#pragma unroll
-  for (int e = 0; e < 4; e++) fine = fine && fabs(z[e]) < __builtin_inf();
-#pragma unroll
-  for (int d = 1; d < 16; d <<= 1) {
-    lo = fmin(lo, __shfl_xor(lo, d, 64));
-    hi = fmax(hi, __shfl_xor(hi, d, 64));
-  }
-  const uint64_t ok = __ballot(fine) >> (threadIdx.x & 48);
-  const double scale = (double)f64_to_f16((hi - lo) / 15.0);
+// Codes of the lane's four columns z of a row, a group being 16 lanes whose least
+// and largest values are lo and hi and which are all finite (`fine`).
+__device__ __forceinline__ Quant quantise(const double (&z)[4], double lo, double hi, bool fine) {
+  // (hi - lo) / 15, as a division rounds it: the second product makes up what the
+  // reciprocal lacks
+  const double range = hi - lo, q = range * (1.0 / 15.0);
+  const double scale = (double)f64_to_f16(fma(fma(-15.0, q, range), 1.0 / 15.0, q));
   const double offset = (double)f64_to_f16(lo - 16.0 * scale);
-  Quant r;
+  const uint64_t ok = __ballot(fine) >> (threadIdx.x & 48);
   if ((ok & 0xffff) != 0xffff || !(fabs(offset) < __builtin_inf()) || !(scale < __builtin_inf())) {
     const _Float16 bad = (_Float16)__builtin_nanf("");
     return Quant{0, f16x2{bad, bad}};
   }
-  r.codes = 0;
+  // (z - offset) / scale rounded: by the reciprocal, which is off by less than 2^-40,
+  // and where that could be the other side of a tie by the sign of what lies beyond it
+  double inv = __builtin_amdgcn_rcp(scale);
+  inv = fma(fma(-scale, inv, 1.0), inv, inv);
+  inv = fma(fma(-scale, inv, 1.0), inv, inv);
+  double c[4];
+  double far = 0.0;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
-    const double c = scale > 0.0 ? rint((z[e] - offset) / scale) - 16.0 : 0.0;
-    r.codes |= (uint32_t)(int)fmin(fmax(c, 0.0), 15.0) << (8 * e);
+    const double t = (z[e] - offset) * inv;
+    c[e] = rint(t);
+    far = fmax(far, fabs(t - c[e]));
   }
+  if (__any(far > 0.5 - 0x1p-36)) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const double d = z[e] - offset, low = floor(d * inv), beyond = fma(-(low + 0.5), scale, d);
+      if (fabs(beyond) < 0x1p-30 * scale)
+        c[e] = beyond > 0.0 || (beyond == 0.0 && 0.5 * low != floor(0.5 * low)) ? low + 1.0 : low;
+    }
+  }
+  Quant r;
+  r.codes = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    r.codes |= (uint32_t)min(max((int)c[e] - 16, 0), 15) << (8 * e);
+  if (scale == 0.0) r.codes = 0;
   r.so = f16x2{(_Float16)(float)scale, (_Float16)(float)offset};
   return r;
+}
+template <typename T>
+__device__ __forceinline__ Quant quantise(const T (&x)[4]) {
+  T lo = fmin(fmin(x[0], x[1]), fmin(x[2], x[3])), hi = fmax(fmax(x[0], x[1]), fmax(x[2], x[3]));
+  bool fine = true;
+#pragma unroll
+  for (int e = 0; e < 4; e++) fine = fine && __builtin_isfinite(x[e]);
+  lo = mi::over_row(lo, [](T a, T b) { return fmin(a, b); });
+  hi = mi::over_row(hi, [](T a, T b) { return fmax(a, b); });
+  const double z[4] = {(double)x[0], (double)x[1], (double)x[2], (double)x[3]};
+  return quantise(z, (double)lo, (double)hi, fine);
 }
 
 // Four bytes of codes as 16 bits of nibbles.
@@ -141,24 +170,31 @@ __device__ __forceinline__ int find_token(const mi::PagedView& pv, int tok, int&
   return s;
 }
 
-// One query head of one token.
-template <typename T, bool ILV>
-__device__ __forceinline__ void q_row(const AppendArgs& a, int64_t item) {
+// EACH query heads of one token.
+template <typename T, bool ILV, int EACH>
+__device__ __forceinline__ void q_rows(const AppendArgs& a, int64_t item) {
   const int lane = threadIdx.x & 63;
-  const int64_t tok = item / a.H;
+  const int groups = (a.H + EACH - 1) / EACH;
+  const int64_t tok = item / groups;
   if (tok >= a.n) return;
-  const int h = (int)(item - tok * a.H);
-  const float4 x = load_row<T>(a.q, a.q_ts, a.q_hs, tok, h, lane);
+  const int h0 = (int)(item - tok * groups) * EACH;
+  float4 x[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; i++) x[i] = load_row<T>(a.q, a.q_ts, a.q_hs, tok, min(h0 + i, a.H - 1), lane);
   int q0, nq;
   const int s = find_token(a.pv, (int)tok, q0, nq);
   if (s >= a.pv.batch || tok - q0 < 0 || tok - q0 >= nq) return;  // behind the last sequence
   const int pos = a.pv.kv_len[s] - nq + (int)(tok - q0);
-  float y[4] = {x.x, x.y, x.z, x.w};
   mi::LaneTurn<float, ILV> t;
   t.set(a.plan, (double)pos, lane);
-  if (a.q_w) mi::rms_norm<float>(y, a.q_w, a.eps, lane);
-  t.apply(a.plan, y, lane);
-  mi::store4(a.q_out + (tok * a.H + h) * D + 4 * lane, y);
+#pragma unroll
+  for (int i = 0; i < EACH; i++) {
+    if (h0 + i >= a.H) break;  // uniform
+    float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    if (a.q_w) mi::rms_norm<float>(y, a.q_w, a.eps, lane);
+    t.apply(a.plan, y, lane);
+    mi::store4(a.q_out + (tok * a.H + h0 + i) * D + 4 * lane, y);
+  }
 }
 
 // K (kv 0) or V (1) of the one row that sequence s brings.
@@ -175,8 +211,8 @@ __device__ __forceinline__ void one_row(const AppendArgs& a, int64_t item) {
   uint8_t* tile = a.pv.tile(s, h, pos >> 5);
   if (!tile) return;
   const int row = pos & 31, g = lane >> 4;
-  double z[4] = {x.x, x.y, x.z, x.w};
   if (!kv) {
+    double z[4] = {x.x, x.y, x.z, x.w};
     finish_k<ILV>(a, z, (double)pos, lane);
     const Quant r = quantise(z);
     const uint32_t half = nibbles(r.codes), other = __shfl_xor(half, 1, 64);
@@ -186,7 +222,8 @@ __device__ __forceinline__ void one_row(const AppendArgs& a, int64_t item) {
     const int sub = row >> 4, quad = (row >> 2) & 3, i = row & 3, p = 4 * (i + 4 * sub);
     u32x4* const w = (u32x4*)(tile + mi::kVCodes) + g * 64 + 16 * quad + (lane & 15);
     const u32x4 old = *w;
-    const Quant r = quantise(z);
+    const float y[4] = {x.x, x.y, x.z, x.w};
+    const Quant r = quantise(y);
     u32x4 now;
 #pragma unroll
     for (int j = 0; j < 4; j++)
@@ -205,7 +242,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const AppendArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
   if (wg < a.kv_items) one_row<T, ILV>(a, wg * 4 + w);
-  else q_row<T, ILV>(a, (wg - a.kv_items) * 4 + w);
+  else q_rows<T, ILV, 1>(a, (wg - a.kv_items) * 4 + w);
 }
 
 // The tile that item x of a call stands for: sequence s takes items from
@@ -252,24 +289,25 @@ __device__ void one_tile(const AppendArgs& a, int64_t item) {
   const int row0 = it.tile * 32;                  // row of the sequence at row 0 of the tile
   const int r0 = max(it.first - row0, 0);         // the call's rows of the tile: [r0, r1)
   const int r1 = min(it.end - row0, 32);
-  float4 xk[8], xv[8];
+  constexpr int kEach = 32 / kTileWaves;  // rows of a wave
+  float4 xk[kEach], xv[kEach];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {  // rows outside read the nearest inside
-    const int r = min(max(8 * w + i, r0), r1 - 1);
+  for (int i = 0; i < kEach; i++) {  // rows outside read the nearest inside
+    const int r = min(max(kEach * w + i, r0), r1 - 1);
     const int64_t tok = it.q0 + (row0 + r - it.first);
     xk[i] = load_row<T>(a.k, a.k_ts, a.k_hs, tok, h, lane);
     xv[i] = load_row<T>(a.v, a.v_ts, a.v_hs, tok, h, lane);
   }
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int r = 8 * w + i;
+  for (int i = 0; i < kEach; i++) {
+    const int r = kEach * w + i;
     if (r < r0 || r >= r1) continue;  // uniform
     double z[4] = {xk[i].x, xk[i].y, xk[i].z, xk[i].w};
     finish_k<ILV>(a, z, (double)(row0 + r), lane);
     const Quant k = quantise(z);
     const uint32_t half = nibbles(k.codes), other = __shfl_xor(half, 1, 64);
     if (!(lane & 1)) ((uint32_t*)kw)[k_word(r, lane >> 1)] = half | (other << 16);
-    const double u[4] = {xv[i].x, xv[i].y, xv[i].z, xv[i].w};
+    const float u[4] = {xv[i].x, xv[i].y, xv[i].z, xv[i].w};
     const Quant v = quantise(u);
     vc[r][lane] = v.codes;
     if (!(lane & 15)) {
@@ -279,6 +317,7 @@ __device__ void one_tile(const AppendArgs& a, int64_t item) {
   }
   __syncthreads();
   auto mine = [&](int r) { return r >= r0 && r < r1; };
+  if (t >= 256) return;
   if (mine(16 * (t >> 7) + (t & 15))) ((u32x4*)tile)[t] = kw[t];
   if (t < 32 && mine(t)) ((u32x4*)(tile + mi::kKScale))[t] = *(const u32x4*)&ks[t][0];
   {  // V word (g, quad, n, j): t = 64 g + 16 quad + n
@@ -310,10 +349,12 @@ __device__ void one_tile(const AppendArgs& a, int64_t item) {
 }
 
 template <typename T, bool ILV>
-__global__ void __launch_bounds__(256) append_tiles_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(64 * kTileWaves) append_tiles_kernel(const AppendArgs a) {
   const int64_t wg = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (wg < a.kv_items) one_tile<T, ILV>(a, wg);
-  else q_row<T, ILV>(a, (wg - a.kv_items) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+  else if (a.each == 1) q_rows<T, ILV, 1>(a, (wg - a.kv_items) * kTileWaves + w);
+  else q_rows<T, ILV, mi::kRotaryHeads>(a, (wg - a.kv_items) * kTileWaves + w);
 }
 
 template <typename T>
@@ -321,13 +362,16 @@ hipError_t run_append(AppendArgs& a, hipStream_t s) {
   const bool rows = !a.pv.cu_q;
   a.kv_items = rows ? ((int64_t)a.pv.batch * a.pv.G * 2 + 3) / 4
                     : ((int64_t)(a.n >> 5) + 2 * a.pv.batch) * a.pv.G;
-  const int64_t wgs = a.kv_items + (a.q ? ((int64_t)a.n * a.H + 3) / 4 : 0);
+  const int waves = rows ? 4 : kTileWaves;
+  a.each = rows ? 1 : mi::rotary_heads((int64_t)a.n * a.H);
+  const int64_t q_items = a.q ? (int64_t)a.n * ((a.H + a.each - 1) / a.each) : 0;
+  const int64_t wgs = a.kv_items + (q_items + waves - 1) / waves;
   const int64_t gx = std::min<int64_t>(wgs, 1 << 22);
   const auto f = rows ? (a.plan.interleaved ? append_rows_kernel<T, true> : append_rows_kernel<T, false>)
                       : (a.plan.interleaved ? append_tiles_kernel<T, true>
                                             : append_tiles_kernel<T, false>);
-  return mi::launch("paged_append", f, dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)), dim3(256),
-                    0, s, a);
+  return mi::launch("paged_append", f, dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)),
+                    dim3(64 * waves), 0, s, a);
 }
 
 // ------------------------------------------------------------------- read --

@@ -24,6 +24,12 @@ struct RotaryPlan {
   int32_t interleaved;
 };
 
+// Heads of a token that a wave takes in turn, with their angles once: for many rows,
+// where a wave's instructions are what counts (105k f16 rows, 64 pairs: one head 24.9
+// us, 108 MB); with few rows the chain of one wave does.
+constexpr int kRotaryHeads = 4;
+inline int rotary_heads(int64_t rows) { return rows < 16384 ? 1 : kRotaryHeads; }
+
 // Checks and copies the caller's plan (host_freq may be null when rotary_dim
 // is 0).
 mi_status rotary_plan(const double* host_freq, int32_t rotary_dim, int32_t interleaved,
@@ -124,12 +130,32 @@ struct LaneTurn {
   }
 };
 
+// The value N lanes on in the lane's row of 16 (a data-parallel-primitive move, no LDS).
+template <int N, typename T>
+__device__ __forceinline__ T row_turn(T x) {
+  if constexpr (sizeof(T) == 8) {
+    const u32x2 w = __builtin_bit_cast(u32x2, x);
+    const uint32_t lo = w[0], hi = w[1];
+    return __builtin_bit_cast(T, u32x2{(uint32_t)__builtin_amdgcn_mov_dpp((int)lo, 0x120 + N, 0xf, 0xf, true),
+                                       (uint32_t)__builtin_amdgcn_mov_dpp((int)hi, 0x120 + N, 0xf, 0xf, true)});
+  } else {
+    return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x120 + N, 0xf, 0xf, true));
+  }
+}
+// f over the lane's row of 16, in every lane of it.
+template <typename T, typename F>
+__device__ __forceinline__ T over_row(T x, F f) {
+  x = f(x, row_turn<8>(x));
+  x = f(x, row_turn<4>(x));
+  x = f(x, row_turn<2>(x));
+  return f(x, row_turn<1>(x));
+}
 // Sum over a wave.
 template <typename T>
 __device__ __forceinline__ T wave_sum(T x) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-  return x;
+  x = over_row(x, [](T a, T b) { return a + b; });
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
 }
 
 // RMS norm of a head with bf16 weights, in T.

@@ -1,7 +1,7 @@
 // Rotary positions of one tensor, with an optional RMS norm before.
 //
 // Bound: memory for many tokens; the chain of one wave for few.  A wave takes
-// one head (mi::LaneTurn).
+// one head of a token, or four with their angles once (mi::LaneTurn).
 #include "rotary.h"
 
 #include <algorithm>
@@ -16,38 +16,49 @@ struct RopeApplyArgs {
   const void* positions;  // int32 or int64 [n]
   const uint16_t* norm_w;  // bf16 [D] or null
   void* out;              // [n][heads][D]
-  int64_t rows;           // n * heads
-  int32_t heads, pos64;
+  int32_t n, heads, pos64;
   double eps;
   mi::RotaryPlan plan;
 };
 
-template <typename TI, typename TO, bool ILV>
+template <typename TI, typename TO, bool ILV, int EACH>
 __global__ void __launch_bounds__(256) rope_apply_kernel(const RopeApplyArgs a) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 +
-                      __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (row >= a.rows) return;
-  const int64_t tok = row / a.heads;
-  const int head = (int)(row - tok * a.heads);
-  const float4 x = mi::load4((const TI*)a.x + tok * a.ts + head * a.hs + 4 * lane);
+  const int64_t item = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 4 +
+                       __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int groups = (a.heads + EACH - 1) / EACH;
+  const int64_t tok = item / groups;
+  if (tok >= a.n) return;
+  const int h0 = (int)(item - tok * groups) * EACH;
+  float4 x[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; i++)
+    x[i] = mi::load4((const TI*)a.x + tok * a.ts + min(h0 + i, a.heads - 1) * a.hs + 4 * lane);
   const double pos = a.pos64 ? (double)((const int64_t*)a.positions)[tok]
                              : (double)((const int32_t*)a.positions)[tok];
-  float y[4] = {x.x, x.y, x.z, x.w};
   mi::LaneTurn<float, ILV> t;
   t.set(a.plan, pos, lane);
-  if (a.norm_w) mi::rms_norm<float>(y, a.norm_w, a.eps, lane);
-  t.apply(a.plan, y, lane);
-  mi::store4((TO*)a.out + row * mi::kHeadDim + 4 * lane, y);
+#pragma unroll
+  for (int i = 0; i < EACH; i++) {
+    if (h0 + i >= a.heads) break;  // uniform
+    float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+    if (a.norm_w) mi::rms_norm<float>(y, a.norm_w, a.eps, lane);
+    t.apply(a.plan, y, lane);
+    mi::store4((TO*)a.out + (tok * a.heads + h0 + i) * mi::kHeadDim + 4 * lane, y);
+  }
 }
 
 template <typename TI, typename TO>
 hipError_t run(const RopeApplyArgs& a, hipStream_t s) {
-  const int64_t wgs = (a.rows + 3) / 4, gx = std::min<int64_t>(wgs, 1 << 22);
-  return mi::launch("rope_apply",
-                    a.plan.interleaved ? rope_apply_kernel<TI, TO, true>
-                                       : rope_apply_kernel<TI, TO, false>,
-                    dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)), dim3(256), 0, s, a);
+  const int each = mi::rotary_heads((int64_t)a.n * a.heads);
+  const int64_t wgs = ((int64_t)a.n * ((a.heads + each - 1) / each) + 3) / 4;
+  const int64_t gx = std::min<int64_t>(wgs, 1 << 22);
+  const auto f = each == 1 ? (a.plan.interleaved ? rope_apply_kernel<TI, TO, true, 1>
+                                                 : rope_apply_kernel<TI, TO, false, 1>)
+                           : (a.plan.interleaved ? rope_apply_kernel<TI, TO, true, mi::kRotaryHeads>
+                                                 : rope_apply_kernel<TI, TO, false, mi::kRotaryHeads>);
+  return mi::launch("rope_apply", f, dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)), dim3(256), 0, s,
+                    a);
 }
 template <typename TI>
 hipError_t run(const RopeApplyArgs& a, int32_t out_type, hipStream_t s) {
@@ -127,7 +138,7 @@ extern "C" mi_status mi_rope_apply(const void* x, int32_t x_type, int64_t token_
   a.pos64 = positions_64;
   a.norm_w = norm_w;
   a.out = out;
-  a.rows = (int64_t)n * heads;
+  a.n = n;
   a.heads = heads;
   a.eps = eps;
   const hipStream_t s = (hipStream_t)stream;

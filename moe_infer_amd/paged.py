@@ -29,12 +29,14 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .attention import HEAD_DIM, _ptr, _stream
+from .attention import HEAD_DIM, _device, _stream
 from .kv_cache import _cfg_get
 
 TILE_ROWS = 32
 TILE_BYTES = 9216
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_HALF = (torch.float16,)
+_GATES = (torch.float16, torch.float32)
 
 
 class Rope:
@@ -139,10 +141,32 @@ _NO_ROPE = Rope(0)
 
 
 # ----------------------------------------------------------------- checks --
+#
+# A small call is a few us of GPU work and what the host spends decides how fast
+# it goes: each check is one expression while nothing is wrong (0.2 to 0.5 us a
+# tensor against 0.6 to 1.1 one by one), and only then looks for what is.
 
-def _check_rows(name: str, t, n: int | None, heads: int | None, dtypes):
-    """[n, heads, 256] on the current device, its columns contiguous: (token
+def _current() -> int:
+    """The current device; -2, which no tensor is on, where there is none."""
+    try:
+        return _device()
+    except (RuntimeError, AssertionError):
+        return -2
+
+
+def _check_rows(name: str, t, n: int | None, heads: int | None, dtypes, dev: int):
+    """[n, heads, 256] on device dev, its columns contiguous: (tokens, heads, token
     stride, head stride)."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and t.dim() == 3 and t.get_device() == dev:
+        (rows, h, d), (ts, hs, cs) = t.shape, t.stride()
+        if h == 1:
+            hs = HEAD_DIM
+        if rows == 1:
+            ts = h * hs
+        size = t.element_size()
+        if (d == HEAD_DIM and cs == 1 and (n is None or rows == n) and (heads is None or h == heads)
+                and not (t.data_ptr() | ts * size | hs * size) & 15 and hs >= d and ts >= d):
+            return rows, h, ts, hs
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in dtypes:
@@ -153,73 +177,69 @@ def _check_rows(name: str, t, n: int | None, heads: int | None, dtypes):
         raise ValueError(f"{name} has {t.shape[0]} tokens, expected {n}")
     if heads is not None and t.shape[1] != heads:
         raise ValueError(f"{name} has {t.shape[1]} heads, expected {heads}")
-    _check_device(name, t)
-    ts, hs, cs = t.stride()
-    if cs != 1:
+    _refuse_device(name, t, dev)
+    if t.stride(2) != 1:
         raise ValueError(f"{name}: its {HEAD_DIM} columns must be contiguous")
-    if t.shape[1] == 1:
-        hs = HEAD_DIM
-    if t.shape[0] == 1:
-        ts = t.shape[1] * hs
-    size = t.element_size()
-    if (t.data_ptr() | ts * size | hs * size) & 15:
-        raise ValueError(f"{name}: every row must be 16-byte aligned")
+    if t.numel() == 0:
+        raise ValueError(f"{name} is empty")
     if hs < HEAD_DIM or ts < HEAD_DIM:
         raise ValueError(f"{name}: rows overlap (strides {ts}, {hs})")
-    return ts, hs
+    raise ValueError(f"{name}: every row must be 16-byte aligned")
 
 
-def _check_device(name: str, t: torch.Tensor) -> None:
+def _refuse_device(name: str, t: torch.Tensor, dev: int) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor, got {t.device}")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{dev}")
 
 
-def _check_table(name: str, t, numel: int | None, dtype=torch.int32) -> None:
+def _check_table(name: str, t, numel: int | None, dtype, dev: int, aligned: int = 0) -> None:
+    """A contiguous tensor of `dtype` on device dev; aligned: 15 for whole 16 bytes."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.is_contiguous()
+            and (numel is None or t.numel() == numel) and not t.data_ptr() & aligned):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    _check_device(name, t)
+    _refuse_device(name, t, dev)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name} has {t.numel()} elements, expected {numel}")
+    raise ValueError(f"{name} must be 16-byte aligned")
 
 
-def _check_pages(pages, block_table, kv_len, cu_q):
-    """The C arguments of the cache: pages .. batch; and the KV heads."""
-    _check_table("pages", pages, None, torch.uint8)
-    if pages.dim() != 4 or pages.shape[3] != TILE_BYTES or 0 in pages.shape:
+def _check_pages(pages, block_table, kv_len, cu_q, dev: int):
+    """The C arguments of the cache: pages .. batch; the batch; and the KV heads."""
+    _check_table("pages", pages, None, torch.uint8, dev, 15)
+    _check_table("block_table", block_table, None, torch.int32, dev)
+    if pages.dim() != 4 or pages.shape[3] != TILE_BYTES or not pages.numel():
         raise ValueError(f"pages must be [pages, KV heads, page rows / {TILE_ROWS}, {TILE_BYTES}], "
                          f"got {tuple(pages.shape)}")
-    _check_table("block_table", block_table, None)
-    if block_table.dim() != 2 or 0 in block_table.shape:
+    if block_table.dim() != 2 or not block_table.numel():
         raise ValueError(f"block_table must be [batch, pages of a sequence], got "
                          f"{tuple(block_table.shape)}")
-    batch = block_table.shape[0]
-    _check_table("kv_len", kv_len, batch)
+    (num, G, tiles, _), (batch, cols) = pages.shape, block_table.shape
+    _check_table("kv_len", kv_len, batch, torch.int32, dev)
     if cu_q is not None:
-        _check_table("cu_q", cu_q, batch + 1)
-    return (pages.data_ptr(), pages.shape[0], pages.shape[2] * TILE_ROWS, block_table.data_ptr(),
-            block_table.shape[1], kv_len.data_ptr(), _ptr(cu_q), batch), pages.shape[1]
+        _check_table("cu_q", cu_q, batch + 1, torch.int32, dev)
+    return (pages.data_ptr(), num, tiles * TILE_ROWS, block_table.data_ptr(), cols, kv_len.data_ptr(),
+            None if cu_q is None else cu_q.data_ptr(), batch), batch, G
 
 
-def _check_norm(name: str, w) -> None:
-    if w is not None:
-        _check_table(name, w, HEAD_DIM, torch.bfloat16)
-        if w.data_ptr() & 15:
-            raise ValueError(f"{name} must be 16-byte aligned")
+def _check_norm(name: str, w, dev: int):
+    if w is None:
+        return None
+    _check_table(name, w, HEAD_DIM, torch.bfloat16, dev, 15)
+    return w.data_ptr()
 
 
-def _check_out(name: str, out, n: int, heads: int, dtype, device):
+def _check_out(name: str, out, n: int, heads: int, dtype, dev: int):
     if out is None:
-        return torch.empty((n, heads, HEAD_DIM), dtype=dtype, device=device)
-    _check_table(name, out, n * heads * HEAD_DIM, dtype)
-    if out.data_ptr() & 15:
-        raise ValueError(f"{name} must be 16-byte aligned")
+        return torch.empty((n, heads, HEAD_DIM), dtype=dtype, device=dev)
+    _check_table(name, out, n * heads * HEAD_DIM, dtype, dev, 15)
     return out
 
 
@@ -231,24 +251,20 @@ def rope_apply(x: torch.Tensor, positions: torch.Tensor, rope: Rope,
     """x [n, heads, 256] (f32, f16 or bf16, any token and head stride) rotated
     at positions [n] (int32 or int64), after an RMS norm with norm_w (bf16 [256])
     if given.  Returns [n, heads, 256] of out_dtype (default x's); out may be x."""
-    if not isinstance(x, torch.Tensor) or x.dim() != 3:
-        raise TypeError("x must be a tensor [tokens, heads, 256]")
-    n, heads = x.shape[0], x.shape[1]
-    ts, hs = _check_rows("x", x, None, None, _DTYPES)
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64):
-        raise TypeError("positions must be an int32 or int64 tensor")
-    _check_table("positions", positions, n, positions.dtype)
+    dev = _current()
+    n, heads, ts, hs = _check_rows("x", x, None, None, _DTYPES, dev)
+    wide = isinstance(positions, torch.Tensor) and positions.dtype is torch.int64
+    _check_table("positions", positions, n, torch.int64 if wide else torch.int32, dev)
     if not isinstance(rope, Rope):
         raise TypeError("rope must be a Rope")
-    _check_norm("norm_w", norm_w)
+    w = _check_norm("norm_w", norm_w, dev)
     dtype = out_dtype or (out.dtype if out is not None else x.dtype)
     if dtype not in _DTYPES:
         raise TypeError(f"out_dtype {dtype}")
-    out = _check_out("out", out, n, heads, dtype, x.device)
+    out = _check_out("out", out, n, heads, dtype, dev)
     _lib.check(_lib.lib().mi_rope_apply(
-        x.data_ptr(), _DTYPES[x.dtype], ts, hs, n, heads, HEAD_DIM, positions.data_ptr(),
-        positions.dtype == torch.int64, _ptr(norm_w), eps, *rope._args, out.data_ptr(),
-        _DTYPES[dtype], _stream()))
+        x.data_ptr(), _DTYPES[x.dtype], ts, hs, n, heads, HEAD_DIM, positions.data_ptr(), wide, w, eps,
+        *rope._args, out.data_ptr(), _DTYPES[dtype], _stream()))
     return out
 
 
@@ -264,30 +280,29 @@ def paged_append(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.T
     With q [n, H, 256] returns it normed and rotated, [n, H, 256] f16 (q_out; may
     be q).  q, k, v: one of f32, f16, bf16, any token and head stride (a view of a
     projection).  No rope: no rotation."""
-    head, G = _check_pages(pages, block_table, kv_len, cu_q)
-    if not isinstance(k, torch.Tensor) or k.dim() != 3:
-        raise TypeError("k must be a tensor [tokens, KV heads, 256]")
-    n, batch = k.shape[0], head[-1]
+    dev = _current()
+    head, batch, G = _check_pages(pages, block_table, kv_len, cu_q, dev)
+    n, _, kts, khs = _check_rows("k", k, None, G, _DTYPES, dev)
     if cu_q is None and n != batch:
         raise ValueError(f"{n} tokens for {batch} sequences without cu_q")
-    kts, khs = _check_rows("k", k, None, G, _DTYPES)
-    vts, vhs = _check_rows("v", v, n, G, (k.dtype,))
-    _check_norm("q_norm_w", q_norm_w)
-    _check_norm("k_norm_w", k_norm_w)
-    rope = _NO_ROPE if rope is None else rope
-    if not isinstance(rope, Rope):
+    same = (k.dtype,)
+    _, _, vts, vhs = _check_rows("v", v, n, G, same, dev)
+    if rope is None:
+        rope = _NO_ROPE
+    elif not isinstance(rope, Rope):
         raise TypeError("rope must be a Rope")
     H = qts = qhs = 0
+    qp = None
     if q is not None:
-        qts, qhs = _check_rows("q", q, n, None, (k.dtype,))
-        H = q.shape[1]
-        q_out = _check_out("q_out", q_out, n, H, torch.float16, q.device)
+        _, H, qts, qhs = _check_rows("q", q, n, None, same, dev)
+        q_out = _check_out("q_out", q_out, n, H, torch.float16, dev)
+        qp = q.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
     _lib.check(_lib.lib().mi_paged_append(
-        *head, n, H, G, HEAD_DIM, _DTYPES[k.dtype], _ptr(q), qts, qhs, k.data_ptr(), kts, khs,
-        v.data_ptr(), vts, vhs, _ptr(q_norm_w), _ptr(k_norm_w), eps, *rope._args, _ptr(q_out),
-        _stream()))
+        *head, n, H, G, HEAD_DIM, _DTYPES[k.dtype], qp, qts, qhs, k.data_ptr(), kts, khs, v.data_ptr(),
+        vts, vhs, _check_norm("q_norm_w", q_norm_w, dev), _check_norm("k_norm_w", k_norm_w, dev), eps,
+        *rope._args, None if q is None else q_out.data_ptr(), _stream()))
     return q_out
 
 
@@ -297,15 +312,16 @@ def paged_read(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Ten
     """(k, v), each [n, G, 256] f16: the last cu_q[s + 1] - cu_q[s] rows of each
     sequence (without cu_q the last row), as stored.  n: their number, cu_q[-1];
     with cu_q it must be given, so that the call need not wait for the GPU."""
-    head, G = _check_pages(pages, block_table, kv_len, cu_q)
+    dev = _current()
+    head, batch, G = _check_pages(pages, block_table, kv_len, cu_q, dev)
     if n is None:
         if cu_q is not None:
             raise ValueError("n must be given with cu_q")
-        n = head[-1]
+        n = batch
     n = int(n)
     k, v = out if out is not None else (None, None)
-    k = _check_out("k", k, n, G, torch.float16, pages.device)
-    v = _check_out("v", v, n, G, torch.float16, pages.device)
+    k = _check_out("k", k, n, G, torch.float16, dev)
+    v = _check_out("v", v, n, G, torch.float16, dev)
     _lib.check(_lib.lib().mi_paged_read(*head, n, G, HEAD_DIM, k.data_ptr(), v.data_ptr(), _stream()))
     return k, v
 
@@ -323,27 +339,27 @@ def paged_workspace(batch: int, n: int, max_q: int, max_len: int, num_q_heads: i
 
 
 def _attend(pages, block_table, kv_len, cu_q, q, max_q, max_len, gate, out, workspace):
-    head, G = _check_pages(pages, block_table, kv_len, cu_q)
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        raise TypeError("q must be a tensor [tokens, heads, 256]")
-    n, H = q.shape[0], q.shape[1]
-    if cu_q is None and n != head[-1]:
-        raise ValueError(f"{n} tokens for {head[-1]} sequences")
-    qts, qhs = _check_rows("q", q, None, None, (torch.float16,))
+    dev = _current()
+    head, batch, G = _check_pages(pages, block_table, kv_len, cu_q, dev)
+    n, H, qts, qhs = _check_rows("q", q, None, None, _HALF, dev)
+    if cu_q is None and n != batch:
+        raise ValueError(f"{n} tokens for {batch} sequences")
     if H % G:
         raise ValueError(f"{H} query heads for {G} KV heads")
+    gp = None
     g_type = gts = ghs = 0
     if gate is not None:
-        gts, ghs = _check_rows("gate", gate, n, H, (torch.float16, torch.float32))
+        _, _, gts, ghs = _check_rows("gate", gate, n, H, _GATES, dev)
         g_type = _DTYPES[gate.dtype]
-    out = _check_out("out", out, n, H, torch.float16, q.device)
+        gp = gate.data_ptr()
+    out = _check_out("out", out, n, H, torch.float16, dev)
     if workspace is None:
-        workspace = paged_workspace(head[-1], n, max_q, max_len, H, G, q.device)
+        workspace = paged_workspace(batch, n, max_q, max_len, H, G, q.device)
     else:
-        _check_table("workspace", workspace, None, torch.uint8)
+        _check_table("workspace", workspace, None, torch.uint8, dev, 15)
     _lib.check(_lib.lib().mi_attn_paged(
-        *head, n, max_q, max_len, H, G, HEAD_DIM, q.data_ptr(), qts, qhs, _ptr(gate), g_type, gts,
-        ghs, out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream()))
+        *head, n, max_q, max_len, H, G, HEAD_DIM, q.data_ptr(), qts, qhs, gp, g_type, gts, ghs,
+        out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream()))
     return out
 
 
