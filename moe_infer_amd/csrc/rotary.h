@@ -9,6 +9,9 @@
 // their Taylor sums, in f32 to the terms r^9 and r^10 (the next are 2e-9) or in
 // f64 to r^15 and r^16 (5e-17).
 //
+// Products and sums are written as the fused operations they become, so that every
+// kernel rounds a rotation alike.
+//
 // A wave holds one head of 256 columns, lane l the columns 4 l .. 4 l + 3; an
 // angle is computed once, in one lane, and fetched from it.
 #pragma once
@@ -66,7 +69,7 @@ __device__ __forceinline__ void turn(double t, T& s, T& c) {
     pc = fmaf(r2, pc, 1.f / 24.f);
     pc = fmaf(r2, pc, -0.5f);
   }
-  const T sr = r + r * r2 * ps, cr = (T)1 + r2 * pc;
+  const T sr = fma(r * r2, ps, r), cr = fma(r2, pc, (T)1);
   const int quadrant = (int)(k - 4.0 * rint(k * 0.25)) & 3;  // -2 .. 2
   const T a = quadrant & 1 ? cr : sr, b = quadrant & 1 ? sr : cr;
   s = quadrant & 2 ? -a : a;
@@ -112,8 +115,8 @@ struct LaneTurn {
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const T a = y[2 * e], b = y[2 * e + 1];
-          y[2 * e] = a * c[e] - b * s[e];
-          y[2 * e + 1] = b * c[e] + a * s[e];
+          y[2 * e] = fma(a, c[e], -(b * s[e]));
+          y[2 * e + 1] = fma(b, c[e], a * s[e]);
         }
       }
     } else {
@@ -124,7 +127,7 @@ struct LaneTurn {
       for (int e = 0; e < 4; e++) o[e] = __shfl(y[e], partner & 63, 64);
       if (4 * lane < 2 * p.half) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = lower ? y[e] * c[e] - o[e] * s[e] : y[e] * c[e] + o[e] * s[e];
+        for (int e = 0; e < 4; e++) y[e] = fma(y[e], c[e], lower ? -(o[e] * s[e]) : o[e] * s[e]);
       }
     }
   }
@@ -161,7 +164,7 @@ __device__ __forceinline__ T wave_sum(T x) {
 // RMS norm of a head with bf16 weights, in T.
 template <typename T>
 __device__ __forceinline__ void rms_norm(T (&y)[4], const uint16_t* w, double eps, int lane) {
-  const T ss = wave_sum<T>(y[0] * y[0] + y[1] * y[1] + y[2] * y[2] + y[3] * y[3]);
+  const T ss = wave_sum<T>(fma(y[0], y[0], fma(y[1], y[1], fma(y[2], y[2], y[3] * y[3]))));
   T inv;
   if constexpr (sizeof(T) == 8) inv = 1.0 / sqrt(ss / kHeadDim + eps);
   else inv = 1.f / sqrtf(ss / (float)kHeadDim + (float)eps);
