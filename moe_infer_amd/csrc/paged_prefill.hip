@@ -186,32 +186,36 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   u32x4 rk[2], rv[2];
   uint32_t sk, sv;
   bool lost = false;
-  auto base = [&](int t32) -> __amdgpu_buffer_rsrc_t {
-    const uint8_t* p = nullptr;
-    if (t32 * 32 < end) {
-      p = a.pv.tile(s, h, t32);
-      lost = lost || !p;
-    }
+  // Where tiles t + 1, t + 2 and t + 3 lie (at[i][u]: tile 2 (t + i) + u), looked up a tile
+  // before their loads.
+  const uint8_t* at[4][2];
+  auto page = [&](int t32) { return t32 * 32 < end ? a.pv.page(s, t32) : -1; };
+  auto place = [&](int32_t id, int t32) {
+    const uint8_t* p = t32 * 32 < end ? a.pv.at(id, h, t32) : nullptr;
+    lost = lost || (t32 * 32 < end && !p);
+    return p;
+  };
+  auto buffer = [&](const uint8_t* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, p ? mi::kTileBytes : 0,
                                              0x00020000);
   };
   const int m16 = lane & 15, quad = lane >> 4;
   const int su = w >> 1, sat = 4 * (tid & 127);  // the thread's word of scales: tile, offset
-  auto load_k = [&](int t) {
+  auto load_k = [&](int i) {
 #pragma unroll
     for (int u = 0; u < 2; u++)
-      rk[u] = __builtin_amdgcn_raw_buffer_load_b128(base(2 * t + u), 16 * tid, 0, 0);
+      rk[u] = __builtin_amdgcn_raw_buffer_load_b128(buffer(at[i][u]), 16 * tid, 0, 0);
   };
-  auto load_v = [&](int t) {
+  auto load_v = [&](int i) {
 #pragma unroll
     for (int u = 0; u < 2; u++)
-      rv[u] = __builtin_amdgcn_raw_buffer_load_b128(base(2 * t + u), mi::kVCodes + 16 * tid, 0, 0);
+      rv[u] = __builtin_amdgcn_raw_buffer_load_b128(buffer(at[i][u]), mi::kVCodes + 16 * tid, 0, 0);
   };
-  auto load_sk = [&](int t) {
-    sk = __builtin_amdgcn_raw_buffer_load_b32(base(2 * t + su), mi::kKScale + sat, 0, 0);
+  auto load_sk = [&](int i) {
+    sk = __builtin_amdgcn_raw_buffer_load_b32(buffer(su ? at[i][1] : at[i][0]), mi::kKScale + sat, 0, 0);
   };
-  auto load_sv = [&](int t) {
-    sv = __builtin_amdgcn_raw_buffer_load_b32(base(2 * t + su), mi::kVScale + sat, 0, 0);
+  auto load_sv = [&](int i) {
+    sv = __builtin_amdgcn_raw_buffer_load_b32(buffer(su ? at[i][1] : at[i][0]), mi::kVScale + sat, 0, 0);
   };
   const uint32_t x16 = mi::sixteens();
   char* const kbuf = lds;
@@ -247,17 +251,25 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   // V word j: product quad / 2, block 2 w + j / 2, lane half quad % 2, slot 16 (j % 2) + n
   const int vdst = (((quad >> 1) * 8 + 2 * w) * 2 * 32 + (quad & 1) * 32 + m16) * 16;
   const int vsrc = 32 * (4 * w + quad);
+  f16x2 kso[2][2];
+  auto get_ks = [&](int t) {  // a piece's scales, ahead of its words
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+        kso[u][i] = *(const f16x2*)(ksc + (t & 1) * 1024 + 512 * u + ksrc + 4 * i);
+  };
   auto put_k = [&](int t, int u, int j) {
-    const f16x2 so = *(const f16x2*)(ksc + (t & 1) * 1024 + 512 * u + ksrc + 4 * (j >> 1));
+    const f16x2 so = kso[u][j >> 1];
     *(f16x8*)(kbuf + ((t & 1) * 2 + u) * kHalf + kdst + (((j >> 1) * 4 * 2 + (j & 1)) * 32) * 16) =
         mi::dequant_row(rk[u][j], f16x2{so[0], so[0]}, f16x2{so[1], so[1]}, x16);
   };
   f16x8 vs, vo;
+  auto get_vs = [&](int t, int u) {
+    vs = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc);
+    vo = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc + 16);
+  };
   auto put_v = [&](int t, int u, int j) {
-    if (j == 0) {
-      vs = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc);
-      vo = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc + 16);
-    }
     *(f16x8*)(vbuf + ((t & 1) * 2 + u) * kHalf + vdst + ((j >> 1) * 64 + 16 * (j & 1)) * 16) =
         mi::dequant_col(rv[u][j], vs, vo, x16);
   };
@@ -279,28 +291,42 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
     // the first walk's products with no weights read a buffer of zeros
     for (int i = tid; i < 2 * kHalf / 16; i += 256)
       ((u32x4*)(vbuf + ((ta - 1) & 1) * 2 * kHalf))[i] = u32x4{};
-    load_sk(ta);
-    load_k(ta);
+    int32_t id[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) id[i][u] = page(2 * (ta + i) + u);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) at[i][u] = place(id[i][u], 2 * (ta + i) + u);
+    load_sk(0);
+    load_k(0);
     put_sk(ta);
-    load_sk(ta + 1);
-    load_sv(ta);
-    load_v(ta);
+    load_sk(1);
+    load_sv(0);
+    load_v(0);
     __syncthreads();
+    get_ks(ta);
 #pragma unroll
     for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int j = 0; j < 4; j++) put_k(ta, u, j);
-    load_k(ta + 1);
+    load_k(1);
     put_sk(ta + 1);
     put_sv(ta);
-    load_sk(ta + 2);
-    load_sv(ta + 1);
+    load_sk(2);
+    load_sv(1);
   }
   __syncthreads();
   for (int t = ta; t < tz; t++) {
     // K Q^T of tile t; between its products the next tile's K and this tile's V go
     // to LDS (what lies behind the last tile is read as zeros)
     f32x16 sc[2];
+    int32_t id[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) id[u] = page(2 * (t + 4) + u);
+    get_ks(t + 1);
     {
       const char* const kr = kbuf + ((t & 1) * 2 + kp) * kHalf + lane * 16;
       constexpr int kRing = 4;
@@ -319,15 +345,23 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         if (ks + kRing < 16) kf[ks % kRing] = *(const f16x8*)(kr + 1024 * (ks + kRing));
         if (ks < 8) put_k(t + 1, ks >> 2, ks & 3);
         else put_v(t, (ks - 8) >> 2, ks & 3);
+        if (ks == 7) get_vs(t, 0);
+        if (ks == 11) get_vs(t, 1);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     put_sk(t + 2);  // its buffer held tile t's, which the last walk read
     put_sv(t + 1);
-    load_sk(t + 3);
-    load_sv(t + 2);
-    load_v(t + 1);
-    load_k(t + 2);
+    load_sk(3);
+    load_sv(2);
+    load_v(1);
+    load_k(2);
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      at[1][u] = at[2][u];
+      at[2][u] = at[3][u];
+      at[3][u] = place(id[u], 2 * (t + 4) + u);
+    }
     // the products' results are read by ordinary instructions from here on
     asm volatile("s_nop 15\n\ts_nop 3" : "+v"(sc[0]), "+v"(sc[1]));
     const int row0 = kKeys * t + 32 * kp;
