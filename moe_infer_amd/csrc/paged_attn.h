@@ -21,6 +21,10 @@ struct AttnArgs {
   int32_t n, R, max_q, max_len, wgs, ncb, gate32, dsplit;
 };
 
+__device__ __forceinline__ void store4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
+  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * kHeadDim + d) =
+      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+}
 // out of four columns: the gate, then f16.
 __device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
   if (a.gate) {
@@ -35,8 +39,7 @@ __device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, i
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = gate_mul(x[e], g[e]);
   }
-  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * kHeadDim + d) =
-      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+  store4(a, tok, head, d, x);
 }
 
 // Sum over the workgroup and the exclusive prefix of each thread's x.
