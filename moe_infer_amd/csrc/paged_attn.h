@@ -21,75 +21,76 @@ struct AttnArgs {
   int32_t n, R, max_q, max_len, wgs, ncb, gate32, dsplit;
 };
 
-__device__ __forceinline__ void store4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
-  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * kHeadDim + d) =
-      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+// Four values of the gate, from element gi on.
+__device__ __forceinline__ f32x4 gate4(const AttnArgs& a, int64_t gi) {
+  if (a.gate32) return *(const f32x4*)((const float*)a.gate + gi);
+  const f16x4 h = *(const f16x4*)((const _Float16*)a.gate + gi);
+  return f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
 }
+
 // out of four columns: the gate, then f16.
 __device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
   if (a.gate) {
-    const int64_t gi = tok * a.g_ts + head * a.g_hs + d;
-    f32x4 g;
-    if (a.gate32) {
-      g = *(const f32x4*)((const float*)a.gate + gi);
-    } else {
-      const f16x4 h = *(const f16x4*)((const _Float16*)a.gate + gi);
-      g = f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
-    }
+    const f32x4 g = gate4(a, tok * a.g_ts + head * a.g_hs + d);
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = gate_mul(x[e], g[e]);
   }
-  store4(a, tok, head, d, x);
+  *(f16x4*)(a.out + (tok * a.pv.G * a.R + head) * kHeadDim + d) =
+      f16x4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32 | (uint32_t)uniform((int)x));
 }
 
 // Sum over the workgroup and the exclusive prefix of each thread's x.
-template <int NT>
-__device__ __forceinline__ int block_scan(int x, int& before, int* lds) {
+template <int NT, typename T>
+__device__ __forceinline__ T block_scan(T x, T& before, T* lds) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int run = x;
+  T run = x;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int y = __shfl_up(run, d, 64);
+    const T y = __shfl_up(run, d, 64);
     if (lane >= d) run += y;
   }
   __syncthreads();  // lds may hold an earlier scan's
   if (lane == 63) lds[w] = run;
   __syncthreads();
-  int base = 0, total = 0;
+  T base = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < NT / 64; i++) {
     if (i < w) base += lds[i];
     total += lds[i];
   }
   before = base + run - x;
-  return __builtin_amdgcn_readfirstlane(total);
+  return uniform(total);
 }
 
 // The sequence s that holds weight unit `unit(total weight)` of weight(s), and the
-// weight before it; s = 0 where no sequence does.  (The host holds the tiles of a
-// batch, over KV heads and blocks, below 2^31.)
-template <int NT, typename W, typename F>
-__device__ __forceinline__ void find_seq(int batch, W weight, F unit, int& s, int& before) {
-  __shared__ int lds[NT / 64 + 2];
+// weight before it; s = 0 where no sequence does.  (The weights' sum fits T.)
+template <int NT, typename T, typename W, typename F>
+__device__ __forceinline__ void find_seq(int batch, W weight, F unit, int& s, T& before) {
+  __shared__ T lds[NT / 64 + 2];
   const int t = threadIdx.x;
   s = 0;
   before = 0;
   if (batch == 1) {
-    unit(__builtin_amdgcn_readfirstlane(weight(0)));
+    unit(uniform(weight(0)));
     return;
   }
-  int total = 0, pre = 0, x = 0;
+  T total = 0, pre = 0, x = 0;
   for (int c = 0; c < batch; c += NT) {
-    x = c + t < batch ? weight(c + t) : 0;
+    x = c + t < batch ? weight(c + t) : T(0);
     total += block_scan<NT>(x, pre, lds);
   }
-  const int want = unit(total);
+  const T want = unit(total);
   if (want >= total) return;
-  int base = 0;
+  T base = 0;
   for (int c = 0; c < batch; c += NT) {
     if (batch > NT) {  // one pass of a small batch has them already
-      x = c + t < batch ? weight(c + t) : 0;
-      const int sum = block_scan<NT>(x, pre, lds);
+      x = c + t < batch ? weight(c + t) : T(0);
+      const T sum = block_scan<NT>(x, pre, lds);
       if (want >= base + sum) {  // uniform
         base += sum;
         continue;
@@ -102,8 +103,8 @@ __device__ __forceinline__ void find_seq(int batch, W weight, F unit, int& s, in
     break;
   }
   __syncthreads();
-  s = __builtin_amdgcn_readfirstlane(lds[NT / 64]);
-  before = __builtin_amdgcn_readfirstlane(lds[NT / 64 + 1]);
+  s = uniform((int)lds[NT / 64]);
+  before = uniform(lds[NT / 64 + 1]);
 }
 
 // Eight columns of Q in dequant_row's order.

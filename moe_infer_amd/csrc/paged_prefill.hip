@@ -1,24 +1,30 @@
 // Attention over the paged 4-bit cache for many tokens: prompts, and chunks
 // behind cached rows.
 //
-// A workgroup takes 128 rows, the (token, query head of the group) pairs of
-// 128 / R consecutive tokens of one sequence and KV head, and walks the keys
-// that they see in tiles of 64.  The four waves dequantise a tile once into
-// LDS as f16, in MFMA operand order; wave (qb, kp) multiplies rows 64 qb .. + 63
-// with keys 32 kp .. + 31 of it (v_mfma_f32_32x32x16_f16, S^T = K Q^T, O^T += V^T
-// P^T), so that every operand read from LDS feeds two products, and the two
-// key halves join at the end.
+// A workgroup takes blocks of 256 / KP rows, the (token, query head of the group) pairs
+// of consecutive tokens of one sequence and KV head, and walks the keys that they see
+// in tiles of 32 KP.  The four waves dequantise a tile once into LDS as f16, in MFMA
+// operand order; wave (qb, kp) multiplies rows 64 qb .. + 63 with keys 32 kp .. + 31 of
+// it (v_mfma_f32_32x32x16_f16, S^T = K Q^T, O^T += V^T P^T), so that every operand read
+// from LDS feeds two products.  KP = 1: four waves use what is dequantised, 3600 clocks
+// a tile to a wave, 2048 of them MFMA; KP = 2: two do, 4600 clocks, and the two halves of
+// the keys join at the end, but a block is half as long, which is what a sequence of up
+// to 128 rows wants (16 of 128 rows behind 8192: 82 us against 95; 16 of 160: 120
+// against 97; a prompt of 4096 tokens, 512 rows a KV head and 64 tokens: 209 against 197).
 //
-// Bound: the matrix units.  A tile is 64 MFMAs of 32 clocks to a wave, one wave
-// to a SIMD; what else it needs is issued between them: the next tile's
-// dequantisation (16 words a thread) between those of K Q^T, the softmax of tile t
-// between those of P V of tile t - 1.  O^T of 64 rows takes the 256 accumulation
-// registers, so the scores have to come out in ordinary ones: their MFMAs are
-// asm, which the compiler would otherwise give the accumulation form as well.
+// Bound: the instructions that a wave alone on its SIMD issues (535 of four clocks a tile
+// for KP = 1 and 690 for KP = 2, 64 of them MFMAs of 32 clocks).  What a tile needs besides
+// its products is issued between them, each half of a word's dequantisation behind a
+// product of K Q^T, the softmax of tile t behind those of P V of tile t - 1.  O^T of 64
+// rows takes the 256 accumulation registers, so the scores have to come out in ordinary
+// ones: their MFMAs are asm, which the compiler would otherwise give the accumulation form
+// as well.
 //
-// The keys of a block of rows are cut into pieces where one walk would outlast an
-// even share of the call (a few tokens behind a long context): pieces leave
-// partials, paged_prefill_merge_kernel joins them.
+// The keys of all blocks, in the order in which Blocks pairs them, are dealt evenly to one
+// workgroup a CU: ragged batches and causal prompts cost what they hold (chunks behind
+// 2000 to 16000 rows: 366 us against 430 where whole pieces were dealt).  What a share
+// begins and another ends, the merge kernel joins: it reads and writes as much as the
+// partials are, 28 us for 128 blocks of 256 rows.
 #include <algorithm>
 #include <cmath>
 
@@ -30,79 +36,63 @@ using mi::AttnArgs;
 using mi::kNegBig;
 
 constexpr int D = mi::kHeadDim;
-constexpr int kRows = 128;   // rows of a workgroup
-constexpr int kKeys = 64;    // keys of a tile
 constexpr int kHalf = 16384;  // bytes of 32 keys, K or V, as f16
-constexpr int kShare = 256;  // even shares of a call: one per CU
-constexpr int kMinPiece = 8;  // tiles below which keys are not cut further
-constexpr int kSplitBlocks = 256, kSlots = 512;  // most blocks that are cut, and pieces of them
+constexpr int kShares = 256;  // workgroups of a call, one per CU, with an even share each
+constexpr int kOver = 384;    // what starting and ending a block takes, in keys
+// Keys below which shares are not made smaller: 256 against 512, 100 tokens behind 2000
+// rows 40 us and 45, 8 prompts of 100 38 and 48; less than a block's kOver gains nothing.
+constexpr int kMinShare = 256;
 
+// KP: parts of a tile's keys, each another wave's.  256 / KP rows of a block, 32 KP
+// keys of a tile.
+constexpr int rows_of(int kp) { return 256 / kp; }
+
+// What a share leaves to the merge.
+struct Share {
+  int32_t rows, token, head;  // of a block that it begins and does not end: rows (or 0), first
+                              // token, KV head
+  int32_t last, slot;         // the share that ends it, where its own part is
+  int32_t joins;              // its first piece continues a block (in slot 2 share)
+};
 struct PrefillExtra {
-  float* part_o;    // [kSlots][kRows][D]
-  float* part_ml;   // [kSlots][kRows][2]
-  int4* blocks;     // [kSplitBlocks]: sequence, KV head, block, index of its second piece
-  int2* count;      // blocks that are cut, tiles of a piece
+  float* part_o;   // [2 kShares][rows][D]
+  float* part_ml;  // [2 kShares][rows][2]
+  Share* shares;   // [kShares]
 };
 
-// A sequence as blocks of tb tokens.
+// A sequence as blocks of tb tokens.  The walk takes them in pairs, the last with the
+// first and so on inwards: each pair costs the same.
+template <int KP>
 struct Blocks {
   int q0, nq, len, nb, tb;
   bool bad;
   __device__ __forceinline__ int first() const { return len - nq; }
   // rows that block b's last token sees, and tiles of them
   __device__ __forceinline__ int end(int b) const { return first() + min(nq, tb * (b + 1)); }
-  __device__ __forceinline__ int tiles(int b) const { return max(end(b) + kKeys - 1, 0) / kKeys; }
-  // First block with more than x tiles; nb where none has.
-  __device__ __forceinline__ int past(int64_t x) const {
-    if (nb == 0 || len <= x * kKeys) return nb;
-    const int64_t y = x * kKeys - first();
-    return y <= 0 ? 0 : (int)((uint32_t)y / (uint32_t)tb);
+  __device__ __forceinline__ int tiles(int b) const { return max(end(b) + 32 * KP - 1, 32 * KP) / (32 * KP); }
+  // Costs in keys: a block's, a pair's, those of one KV head.
+  __device__ __forceinline__ int64_t cost(int b) const { return (int64_t)max(first(), 0) + kOver + (int64_t)tb * (b + 1); }
+  __device__ __forceinline__ int64_t pair() const { return cost(0) + cost(nb - 1); }
+  __device__ __forceinline__ int64_t all() const { return nb * pair() / 2; }
+  // tiles before x of a block's cost
+  __device__ __forceinline__ int upto(int b, int64_t x) const {
+    const int t = tiles(b);
+    return x >= cost(b) ? t : (int)min((int64_t)t, max(x - kOver, (int64_t)0) / (32 * KP));
   }
 };
-__device__ __forceinline__ Blocks get_blocks(const AttnArgs& a, int s) {
-  Blocks r;
+template <int KP>
+__device__ __forceinline__ Blocks<KP> get_blocks(const AttnArgs& a, int s) {
+  Blocks<KP> r;
   a.pv.tokens(s, r.q0, r.nq);
   r.len = a.pv.kv_len[s];
   r.bad = r.len < 0 || r.len > a.max_len || r.nq > a.max_q;
   if (r.nq <= 0 || r.q0 < 0 || (int64_t)r.q0 + r.nq > a.n) r.nq = 0;
-  r.tb = kRows / a.R;
+  r.tb = rows_of(KP) / a.R;
   r.nb = r.bad ? 0 : (r.nq + r.tb - 1) / r.tb;
   return r;
 }
-// Pieces of a sequence's blocks (one KV head), each of at most `piece` tiles:
-// piece k of block b exists where b >= past(k piece), piece 0 always.  Those of
-// k >= 1 alone with `more`.
-__device__ __forceinline__ int pieces(const Blocks& q, int piece, bool more) {
-  int n = more ? 0 : q.nb;
-  if (q.nb == 0) return 0;
-  const int most = q.tiles(q.nb - 1);
-  for (int64_t x = piece; x < most; x += piece) n += q.nb - q.past(x);
-  return n;
-}
-
-template <int NT>
-__device__ __forceinline__ double block_sum(double x, double* lds) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-  __syncthreads();
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < NT / 64; i++) sum += lds[i];
-  return sum;
-}
-
-// Tiles of a piece: an even share of the call's tiles (at least, so that no more
-// than kShare pieces come on top of one per block), or kMinPiece.
-__device__ __forceinline__ int piece_tiles(const AttnArgs& a, double* lds) {
-  double mine = 0.0;
-  for (int s = threadIdx.x; s < a.pv.batch; s += 256) {
-    const Blocks q = get_blocks(a, s);
-    if (q.nb) mine += (double)q.nb * (0.5 * (q.tiles(0) + q.tiles(q.nb - 1)) + 1.0);
-  }
-  const double all = block_sum<256>(mine, lds) * a.pv.G;
-  return __builtin_amdgcn_readfirstlane(max(kMinPiece, (int)ceil(all / kShare)));
+__device__ __forceinline__ int64_t divide(int64_t x, int64_t y) {  // of what is not negative
+  return (x | y) >> 32 ? x / y : (int64_t)((uint32_t)x / (uint32_t)y);
 }
 
 __device__ __forceinline__ void mfma_s(f32x16& c, f16x8 a, f16x8 b) {
@@ -112,73 +102,87 @@ __device__ __forceinline__ void mfma_s0(f32x16& c, f16x8 a, f16x8 b) {
   asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
 }
 
+template <int KP>
 __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a, const PrefillExtra x) {
   extern __shared__ char lds[];  // K, V [2][2 halves], their scales; then the join of the key halves
-  __shared__ double sums[4];
   __shared__ int odd_row[4];  // least masked row whose V group is not finite
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, hl = lane >> 5;
-  const int qb = w & 1, kp = w >> 1;
-  const int bid = blockIdx.y * gridDim.x + blockIdx.x;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int kRows = rows_of(KP), kKeys = 32 * KP;
+  const int qb = KP == 1 ? w : w & 1, kp = KP == 1 ? 0 : w >> 1;
   const int G = a.pv.G;
+  // Neighbouring shares, which read the same keys, to the CUs of one XCD.
+  const int share = (blockIdx.x & 7) * (kShares / 8) + (blockIdx.x >> 3);
 
-  // ---- which block of which sequence, and which of its tiles
-  const int piece = piece_tiles(a, sums);
-  int s, before, local = -1;
+  int s;
+  int64_t before, at_cost = 0, size = 0, stop = 0;
   mi::find_seq<256>(
-      a.pv.batch, [&](int i) { return pieces(get_blocks(a, i), piece, false); },
-      [&](int total) {
-        local = (uint32_t)bid < (uint32_t)total * (uint32_t)G ? bid : -1;
-        return local < 0 ? total : (int)((uint32_t)bid / (uint32_t)G);
+      a.pv.batch,
+      [&](int i) {
+        const auto q = get_blocks<KP>(a, i);
+        return q.nb ? G * q.all() : (int64_t)0;
+      },
+      [&](int64_t total) {
+        size = max((total + kShares - 1) / kShares, (int64_t)kMinShare);
+        at_cost = min(share * size, total);
+        stop = min(at_cost + size, total);
+        return at_cost;
       },
       s, before);
-  if (bid == 0) {  // for the merge
-    double cut = 0.0;
-    for (int i = tid; i < a.pv.batch; i += 256) {
-      const Blocks q = get_blocks(a, i);
-      cut += q.nb - q.past(piece);
-    }
-    cut = block_sum<256>(cut, sums);
-    if (tid == 0) *x.count = int2{(int)cut * G, piece};
+  const int64_t start = at_cost;
+  Share left{0, 0, 0, 0, 0, 0};
+  while (at_cost < stop) {
+  // ---- the next block, and which of its tiles
+  auto q = get_blocks<KP>(a, s);
+  q.q0 = mi::uniform(q.q0);
+  q.nq = mi::uniform(q.nq);
+  q.len = mi::uniform(q.len);
+  q.nb = mi::uniform(q.nb);
+  const int64_t all = q.nb ? q.all() : 0;
+  if (at_cost - before >= G * all) {
+    before += G * all;
+    s++;
+    continue;
   }
-  if (local < 0) return;
-  Blocks q = get_blocks(a, s);
-  q.q0 = __builtin_amdgcn_readfirstlane(q.q0);
-  q.nq = __builtin_amdgcn_readfirstlane(q.nq);
-  q.len = __builtin_amdgcn_readfirstlane(q.len);
-  q.nb = __builtin_amdgcn_readfirstlane(q.nb);
-  const int per = __builtin_amdgcn_readfirstlane(pieces(q, piece, false));
-  local -= G * before;
-  const int h = (int)((uint32_t)local / (uint32_t)per);
-  local -= h * per;
-  int k = 0, b0 = 0;  // piece k of the blocks from b0 on, the last (longest) first
-  while (local >= q.nb - b0) {
-    local -= q.nb - b0;
-    k++;
-    b0 = __builtin_amdgcn_readfirstlane(q.past((int64_t)k * piece));
+  const int h = (int)divide(at_cost - before, all);
+  int64_t x0 = at_cost - before - h * all;  // of the head's cost, then of the block's
+  const int pair = (int)divide(x0, q.pair());
+  x0 -= pair * q.pair();
+  int b = q.nb - 1 - pair;
+  if (x0 >= q.cost(b)) {
+    x0 -= q.cost(b);
+    b = pair;
   }
-  const int b = q.nb - 1 - local;
+  const int64_t begin = at_cost - x0, full = q.cost(b);
+  at_cost = min(stop, begin + full);
+  const int ta = q.upto(b, x0), tz = q.upto(b, at_cost - begin);
+  if (ta == tz) continue;
+  const bool whole = ta == 0 && tz == q.tiles(b);
+  const int slot = 2 * share + (begin + x0 != start);
   const int tok0 = b * q.tb, ntok = min(q.tb, q.nq - tok0), nrows = ntok * a.R;
-  const int nt_all = q.tiles(b), cuts = max(1, (nt_all + piece - 1) / piece);
+  if (ta != 0) left.joins = 1;
+  else if (!whole) left = Share{nrows, q.q0 + tok0, h, (int)divide(begin + full - 1, size), slot, left.joins};
   const int first = q.first() + tok0;  // row of the block's first token
   const int end = first + ntok;
-  const int ta = (int)((int64_t)nt_all * k / cuts), tz = (int)((int64_t)nt_all * (k + 1) / cuts);
 
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // nothing that hangs on it is kept in registers over blocks
+  const int lane = tid & 63, col = lane & 31, hl = lane >> 5;
+  __syncthreads();  // the last block is out of LDS
   if (tid < 4) odd_row[tid] = INT32_MAX;
 
-  // ---- a tile's words: those of the 32-row tiles 2 t and 2 t + 1.  A thread takes a
-  // 16-byte piece of K and of V of each, and one word of the scales of one of them,
-  // which go through LDS a tile earlier (in registers every thread would hold 20
-  // words of them).
-  u32x4 rk[2], rv[2];
+  // ---- a tile's words: those of KP 32-row tiles.  A thread takes a 16-byte piece of K
+  // and of V of each, and a word of the scales of one of them (of K and of V each, or of
+  // K in the lower waves and of V in the upper), which go through LDS a tile earlier (in
+  // registers every thread would hold 20 words of them).
+  u32x4 rk[KP], rv[KP];
   uint32_t sk, sv;
   bool lost = false;
-  // Where tiles t + 1, t + 2 and t + 3 lie (at[i][u]: tile 2 (t + i) + u), looked up a tile
+  // Where tiles t + 1, t + 2 and t + 3 lie (at[i][u]: 32-row tile KP (t + i) + u), looked up a tile
   // before their loads; the page's id is loaded two tiles before that, by a vector load
   // (a scalar one would hold up every wait for LDS until it has come).  What has no
   // place (behind the last row; a page that the pool does not have, which is lost)
   // reads page 0, and counts for nothing.
-  const uint8_t* at[4][2];
+  const uint8_t* at[4][KP];
   const int pt = a.pv.page_shift - 5;
   const int tend = (end + 31) >> 5;  // 32-row tiles
   const int tlim = (int)min((int64_t)tend, (int64_t)a.pv.cols << pt);
@@ -186,16 +190,16 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   const uint64_t page_bytes = ((uint64_t)a.pv.G << pt) * mi::kTileBytes;
   const uint8_t* const pages = a.pv.pages + ((uint64_t)h << pt) * mi::kTileBytes;
   const int32_t* const table = a.pv.table + (int64_t)s * a.pv.cols;
-  auto ids = [&](int t) {  // lane u's: page of tile 2 t + u, or any where there is none
-    return table[min((2 * t + (lane & 1)) >> pt, a.pv.cols - 1)];
+  auto ids = [&](int t) {  // lane u's: page of tile KP t + u, or any where there is none
+    return table[min((KP * t + (lane & (KP - 1))) >> pt, a.pv.cols - 1)];
   };
-  auto place = [&](const uint8_t* (&p)[2], int32_t idv, int t) {
+  auto place = [&](const uint8_t* (&p)[KP], int32_t idv, int t) {
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < KP; u++) {
       const uint32_t id = __builtin_amdgcn_readlane(idv, u);
-      const int ok = (2 * t + u < tlim) & (id < npages);
-      lost = lost | ((2 * t + u < tend) & (ok ^ 1));
-      const uint64_t off = id * page_bytes + (uint32_t)(((2 * t + u) & ((1 << pt) - 1)) * mi::kTileBytes);
+      const int ok = (KP * t + u < tlim) & (id < npages);
+      lost = lost | ((KP * t + u < tend) & (ok ^ 1));
+      const uint64_t off = id * page_bytes + (uint32_t)(((KP * t + u) & ((1 << pt) - 1)) * mi::kTileBytes);
       p[u] = pages + (ok ? off : 0);
     }
   };
@@ -204,27 +208,29 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   auto buffer = [&](const uint8_t* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, mi::kTileBytes, 0x00020000);
   };
-  auto load_k = [&](u32x4 (&r)[2], int i) {
+  auto load_k = [&](u32x4 (&r)[KP], int i) {
 #pragma unroll
-    for (int u = 0; u < 2; u++) r[u] = __builtin_amdgcn_raw_buffer_load_b128(buffer(at[i][u]), 16 * tid, 0, 0);
+    for (int u = 0; u < KP; u++) r[u] = __builtin_amdgcn_raw_buffer_load_b128(buffer(at[i][u]), 16 * tid, 0, 0);
   };
-  auto load_v = [&](u32x4 (&r)[2], int i) {
+  auto load_v = [&](u32x4 (&r)[KP], int i) {
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int u = 0; u < KP; u++)
       r[u] = __builtin_amdgcn_raw_buffer_load_b128(buffer(at[i][u]), 16 * tid, mi::kVCodes, 0);
   };
   auto load_sk = [&](int i) {
-    return __builtin_amdgcn_raw_buffer_load_b32(buffer(su ? at[i][1] : at[i][0]), sat, mi::kKScale, 0);
+    return __builtin_amdgcn_raw_buffer_load_b32(buffer(KP == 2 && su ? at[i][KP - 1] : at[i][0]), sat,
+                                                mi::kKScale, 0);
   };
   auto load_sv = [&](int i) {
-    return __builtin_amdgcn_raw_buffer_load_b32(buffer(su ? at[i][1] : at[i][0]), sat, mi::kVScale, 0);
+    return __builtin_amdgcn_raw_buffer_load_b32(buffer(KP == 2 && su ? at[i][KP - 1] : at[i][0]), sat,
+                                                mi::kVScale, 0);
   };
   const uint32_t x16 = mi::sixteens();
   char* const kbuf = lds;
-  char* const vbuf = lds + 4 * kHalf;
-  char* const ksc = lds + 8 * kHalf;  // [2][2 tiles][512]
-  char* const vsc = ksc + 2048;
-  auto put_sk = [&](int t, uint32_t y) { *(uint32_t*)(ksc + (t & 1) * 1024 + 4 * tid) = y; };
+  char* const vbuf = lds + 2 * KP * kHalf;
+  char* const ksc = lds + 8 * kHalf;  // [2][KP][512]
+  char* const vsc = ksc + 1024 * KP;
+  auto put_sk = [&](int t, uint32_t y) { *(uint32_t*)(ksc + (t & 1) * 512 * KP + (KP == 2 ? 4 * tid : sat)) = y; };
   // V's word: scale or offset of rows 4 quad + i and 16 more, of group g.  Rows that no
   // token of the block sees read as zero, and so does what is not finite in rows that
   // some token does not see (the MFMA would make NaN of 0 * NaN for it); the
@@ -234,7 +240,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
       int x = tid;
       asm volatile("" : "+v"(x));  // nothing of this is kept in registers over the tiles
       const int i = x & 3, sq = (x >> 3) & 3, g = (x >> 5) & 3;
-      const int row = kKeys * t + 32 * su + 4 * sq + i;
+      const int row = kKeys * t + (KP == 2 ? 32 * su : 0) + 4 * sq + i;
       y &= (row < end ? 0xffffu : 0u) | (row + 16 < end ? 0xffff0000u : 0u);
       const uint32_t odd = ((y & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
       if (odd) {
@@ -242,7 +248,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         y &= ~((odd >> 15) * 0xffffu);
       }
     }
-    *(uint32_t*)(vsc + (t & 1) * 1024 + 4 * tid) = y;
+    *(uint32_t*)(vsc + (t & 1) * 512 * KP + (KP == 2 ? 4 * tid : sat)) = y;
   };
   // The wave's pieces of K: rows 16 (w / 2) + m16, groups 2 (w % 2) and the next.  Word j:
   // operand 4 (2 (w % 2) + j / 2) + quad, lane half j % 2, and the slot whose score lands
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   auto get_ks = [&](int t, int u) {  // a piece's scales, ahead of its words
 #pragma unroll
     for (int i = 0; i < 2; i++)
-      kso[i] = *(const f16x2*)(ksc + (t & 1) * 1024 + 512 * u + ksrc + 4 * i);
+      kso[i] = *(const f16x2*)(ksc + (t & 1) * 512 * KP + 512 * u + ksrc + 4 * i);
   };
   // A word in two halves of six instructions, for the two products of a step.
   f16x2 half[2];
@@ -275,13 +281,13 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
     const f16x2 so = kso[j >> 1], sc = f16x2{so[0], so[0]}, of = f16x2{so[1], so[1]};
     const f16x2 c = mi::pk_fma(mi::codes16<2>(y, x16), sc, of);
     const f16x2 d = mi::pk_fma(mi::codes16<3>(y, x16), sc, of);
-    *(f16x8*)(kbuf + ((t & 1) * 2 + u) * kHalf + kdst + (((j >> 1) * 4 * 2 + (j & 1)) * 32) * 16) =
+    *(f16x8*)(kbuf + ((t & 1) * KP + u) * kHalf + kdst + (((j >> 1) * 4 * 2 + (j & 1)) * 32) * 16) =
         f16x8{half[0][0], half[0][1], half[1][0], half[1][1], c[0], c[1], d[0], d[1]};
   };
   f16x8 vs, vo;
   auto get_vs = [&](int t, int u) {
-    vs = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc);
-    vo = *(const f16x8*)(vsc + (t & 1) * 1024 + 512 * u + vsrc + 16);
+    vs = *(const f16x8*)(vsc + (t & 1) * 512 * KP + 512 * u + vsrc);
+    vo = *(const f16x8*)(vsc + (t & 1) * 512 * KP + 512 * u + vsrc + 16);
   };
   auto half_v = [&](uint32_t y) {
     half[0] = mi::pk_fma(mi::codes16<0>(y, x16), f16x2{vs[0], vs[1]}, f16x2{vo[0], vo[1]});
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   auto put_v = [&](uint32_t y, int t, int u, int j) {
     const f16x2 c = mi::pk_fma(mi::codes16<2>(y, x16), f16x2{vs[4], vs[5]}, f16x2{vo[4], vo[5]});
     const f16x2 d = mi::pk_fma(mi::codes16<3>(y, x16), f16x2{vs[6], vs[7]}, f16x2{vo[6], vo[7]});
-    *(f16x8*)(vbuf + ((t & 1) * 2 + u) * kHalf + vdst + ((j >> 1) * 64 + 16 * (j & 1)) * 16) =
+    *(f16x8*)(vbuf + ((t & 1) * KP + u) * kHalf + vdst + ((j >> 1) * 64 + 16 * (j & 1)) * 16) =
         f16x8{half[0][0], half[0][1], half[1][0], half[1][1], c[0], c[1], d[0], d[1]};
   };
 
@@ -302,41 +308,37 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   f16x8 qf[2][16];
   int lim[2];  // rows of the cache that they see
   int32_t id[4], idn = 0;  // pages of tile t + 4
-  u32x4 k0[2];
+  u32x4 k0[KP];
   uint32_t sk0 = 0, sk1 = 0, sv0 = 0;
-  if (ta < tz) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) id[i] = ids(ta + i);
-    idn = ids(ta + 4);
-  }
+  for (int i = 0; i < 4; i++) id[i] = ids(ta + i);
+  idn = ids(ta + 4);
   const float rinv = 1.f / (float)a.R;
   auto token = [&](int r) { return (int)(((float)r + 0.5f) * rinv); };  // r / R: r < 128
   {
-    f16x8 y[16];
+    f16x8 y[kRows / 8];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int r = 32 * w + 2 * i + hl, rr = r < nrows ? r : 0, tok = token(rr);
+    for (int i = 0; i < kRows / 8; i++) {
+      const int r = kRows / 4 * w + 2 * i + hl, rr = r < nrows ? r : 0, tok = token(rr);
       y[i] = *(const f16x8*)(a.q + (int64_t)(q.q0 + tok0 + tok) * a.q_ts +
                              (h * a.R + rr - tok * a.R) * a.q_hs + 8 * col);
     }
-    if (ta < tz) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) place(at[i], id[i], ta + i);
+    for (int i = 0; i < 4; i++) place(at[i], id[i], ta + i);
+    if (KP == 2 || !su) {
       sk0 = load_sk(0);
       sk1 = load_sk(1);
-      sv0 = load_sv(0);
-      load_k(k0, 0);
-      load_v(rv, 0);
-      load_k(rk, 1);
-      sk = load_sk(2);
-      sv = load_sv(1);
     }
-    // the first walk's products with no weights read a buffer of zeros
-    for (int i = tid; i < 2 * kHalf / 16; i += 256)
-      ((u32x4*)(vbuf + ((ta - 1) & 1) * 2 * kHalf))[i] = u32x4{};
+    if (KP == 2 || su) sv0 = load_sv(0);
+    load_k(k0, 0);
+    load_v(rv, 0);
+    load_k(rk, 1);
+    if (KP == 2 || !su) sk = load_sk(2);
+    if (KP == 2) sv = load_sv(1);
+    else if (su) sk = load_sv(1);
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const int r = 32 * w + 2 * i + hl;
+    for (int i = 0; i < kRows / 8; i++) {
+      const int r = kRows / 4 * w + 2 * i + hl;
       *(f16x8*)(kbuf + 512 * r + 16 * (col ^ (r & 7))) = mi::in_order(y[i]);
     }
   }
@@ -352,19 +354,27 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
 #pragma unroll
   for (int c = 0; c < 2; c++)
 #pragma unroll
-    for (int i = 0; i < 8; i++) acc[c][i] = f32x16{};
+    for (int i = 0; i < 8; i++) {
+      acc[c][i] = f32x16{};
+      asm volatile("" : "+a"(acc[c][i]));
+    }
   f16x8 p[2][2];
 #pragma unroll
   for (int c = 0; c < 2; c++)
 #pragma unroll
     for (int i = 0; i < 2; i++) p[c][i] = f16x8{};
 
-  put_sk(ta, sk0);
-  put_sk(ta + 1, sk1);
+  if (KP == 2 || !su) {
+    put_sk(ta, sk0);
+    put_sk(ta + 1, sk1);
+  }
   __syncthreads();
-  put_sv(ta, sv0);
+  // the first walk's products with no weights read a buffer of zeros
+  for (int i = tid; i < KP * kHalf / 16; i += 256)
+    ((u32x4*)(vbuf + ((ta - 1) & 1) * KP * kHalf))[i] = u32x4{};
+  if (KP == 2 || su) put_sv(ta, sv0);
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
+  for (int u = 0; u < KP; u++) {
     get_ks(ta, u);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -377,7 +387,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   constexpr int kRing = 4;
   f16x8 ring[kRing];
   auto get = [&](const char* buf, int t, int i) {
-    ring[i % kRing] = *(const f16x8*)(buf + ((t & 1) * 2 + kp) * kHalf + opnd + 1024 * i);
+    ring[i % kRing] = *(const f16x8*)(buf + ((t & 1) * KP + kp) * kHalf + opnd + 1024 * i);
   };
   for (int t = ta; t < tz; t++) {
     // K Q^T of tile t; between its products the next tile's K and this tile's V go
@@ -392,22 +402,33 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         if (ks == 0) mfma_s0(sc[0], ring[0], qf[0][0]);
         else mfma_s(sc[0], ring[ks % kRing], qf[0][ks]);
         __builtin_amdgcn_sched_barrier(0);
-        const uint32_t y = ks < 8 ? rk[ks >> 2][ks & 3] : rv[(ks - 8) >> 2][ks & 3];
-        if (ks < 8) half_k(y, ks & 3);
-        else half_v(y);
+        // half of a word here and half behind the other product, or a word every other step
+        const int x = KP == 2 ? ks : ks >> 1, u = x / 4 % KP;
+        const bool isk = x < 4 * KP, one = KP == 2 || ks % 2 == 0, two = KP == 2 || ks % 2 == 1;
+        const uint32_t y = isk ? rk[u][x & 3] : rv[u][x & 3];
+        if (one) {
+          if (isk) half_k(y, x & 3);
+          else half_v(y);
+        }
+        if (KP == 1 && two) {
+          if (isk) put_k(y, t + 1, u, x & 3);
+          else put_v(y, t, u, x & 3);
+        }
         __builtin_amdgcn_sched_barrier(0);
         if (ks == 0) mfma_s0(sc[1], ring[0], qf[1][0]);
         else mfma_s(sc[1], ring[ks % kRing], qf[1][ks]);
         if (ks + kRing < 16) get(kbuf, t, ks + kRing);
         else get(vbuf, t - 1, ks + kRing - 16);
-        if (ks < 8) put_k(y, t + 1, ks >> 2, ks & 3);
-        else put_v(y, t, (ks - 8) >> 2, ks & 3);
-        if (ks == 3) get_ks(t + 1, 1);
+        if (KP == 2) {
+          if (isk) put_k(y, t + 1, u, x & 3);
+          else put_v(y, t, u, x & 3);
+          if (ks == 3) get_ks(t + 1, KP - 1);
+        }
         if (ks == 7) {
           get_vs(t, 0);
           load_k(rk, 2);
         }
-        if (ks == 11) get_vs(t, 1);
+        if (KP == 2 && ks == 11) get_vs(t, KP - 1);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -419,14 +440,20 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
       __builtin_amdgcn_sched_barrier(0);
     };
     product(0, 0);
-    put_sk(t + 2, sk);  // its buffer held tile t's, which the last walk read
-    put_sv(t + 1, sv);
+    if (KP == 2 || !su) put_sk(t + 2, sk);  // its buffer held tile t's, which the last walk read
+    if (KP == 2) put_sv(t + 1, sv);
+    else if (su) put_sv(t + 1, sk);
     load_v(rv, 1);
     product(0, 1);
-    sk = load_sk(3);
-    sv = load_sv(2);
+    if constexpr (KP == 2) {
+      sk = load_sk(3);
+      sv = load_sv(2);
+    } else {
+      sk = __builtin_amdgcn_raw_buffer_load_b32(buffer(su ? at[2][0] : at[3][0]), sat,
+                                                su ? mi::kVScale : mi::kKScale, 0);
+    }
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < KP; u++) {
       at[1][u] = at[2][u];
       at[2][u] = at[3][u];
     }
@@ -511,28 +538,35 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
       }
     mi::sync_lds();
   }
-  // The rows that the wave finishes, and their gates: f16 gates are loaded here, ahead of
-  // the stores that a later load would wait for.
-  const int r0 = 64 * qb + 32 * kp;
-  auto out_row = [&](int i, int64_t& tok, int& head) {
-    const int rr = max(0, min(r0 + i, nrows - 1));
-    const int at = __builtin_amdgcn_readfirstlane(token(rr));
-    tok = q.q0 + tok0 + at;
-    head = h * a.R + rr - at * a.R;
+  const bool early = whole && a.gate && !a.gate32;
+  int r0 = 64 * qb + 32 * kp;
+  // Lane i's: where row r0 + i (or the last one) lies in the gate and in the output.
+  int64_t gate_at, out_at;
+  auto find_rows = [&] {
+    const int r = max(0, min(r0 + col, nrows - 1)), tok = token(r), head = h * a.R + r - tok * a.R;
+    gate_at = (q.q0 + tok0 + tok) * a.g_ts + head * a.g_hs;
+    out_at = ((int64_t)(q.q0 + tok0 + tok) * G * a.R + head) * D;
   };
-  const bool early = cuts == 1 && a.gate && !a.gate32;
+  auto lane64 = [](int64_t x, int i) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)x, i));
+  };
   f16x4 gates[32];
-  if (early) {
+  // f16 gates are loaded ahead of the stores that a later load would wait for.
+  auto load_gates = [&] {
+    find_rows();
+    if (early) {
 #pragma unroll
-    for (int i = 0; i < 32; i++) {
-      int64_t tok;
-      int head;
-      out_row(i, tok, head);
-      gates[i] = *(const f16x4*)((const _Float16*)a.gate + tok * a.g_ts + head * a.g_hs + 4 * lane);
+      for (int i = 0; i < 32; i++)
+        gates[i] = *(const f16x4*)((const _Float16*)a.gate + lane64(gate_at, i) + 4 * lane);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; i++) asm("" : "=v"(gates[i]));  // or the last block's would be kept
     }
-  }
-  if (ta < tz) {
-    const char* const vr = vbuf + (((tz - 1) & 1) * 2 + kp) * kHalf + opnd;
+  };
+  load_gates();
+  {
+    const char* const vr = vbuf + (((tz - 1) & 1) * KP + kp) * kHalf + opnd;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
       const f16x8 vf = *(const f16x8*)(vr + 1024 * i);
@@ -541,19 +575,22 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         acc[c][i & 7] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[c][i >> 3], acc[c][i & 7], 0, 0, 0);
     }
   }
-
-  // ---- the key halves join: wave (qb, kp) finishes rows 32 kp of its 64 and hands
-  // the others to its partner.
 #pragma unroll
   for (int c = 0; c < 2; c++) {
     l[c] = mi::sum_xor32(l[c]);
     if (lost) l[c] = __builtin_nanf("");
   }
   __syncthreads();  // every wave is done with the tiles
-  f32x4* const box = (f32x4*)lds;                    // [2 qb][2 kp][32][64]
-  float2* const mlbox = (float2*)(box + 4 * 32 * 64);  // [2][2][32]
-  {
+
+  // ---- the parts of the keys join: wave (qb, kp) finishes rows 32 kp of its 64 and hands
+  // the others to its partner.
+  f32x4* const box = (f32x4*)lds;  // a wave's [32][64]
+  f32x4* const mine = box + (KP * qb + kp) * 32 * 64;
+  if constexpr (KP == 2) {
+    float2* const mlbox = (float2*)(box + 4 * 32 * 64);  // [2][2][32]
     f32x4* const dst = box + (2 * qb + 1 - kp) * 32 * 64;
+#pragma unroll
+    for (int i = 0; i < 8; i++) asm volatile("" : "+a"(acc[0][i]), "+a"(acc[1][i]));
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
@@ -561,162 +598,184 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         dst[(i * 4 + e4) * 64 + lane] = f32x4{acc[1][i][4 * e4], acc[1][i][4 * e4 + 1],
                                               acc[1][i][4 * e4 + 2], acc[1][i][4 * e4 + 3]};
     if (hl == 0) mlbox[(2 * qb + 1 - kp) * 32 + col] = float2{m[1], l[1]};
-  }
-  mi::sync_lds();
-  const f32x4* const src = box + (2 * qb + kp) * 32 * 64;
-  const float2 ml = mlbox[(2 * qb + kp) * 32 + col];
-  const float top = fmaxf(m[0], ml.x);
-  float fa = __builtin_amdgcn_exp2f(m[0] - top), fb = __builtin_amdgcn_exp2f(ml.x - top);
-  const float sum = l[0] * fa + ml.y * fb;
-  const int r = 64 * qb + 32 * kp + col;
-  if (cuts == 1) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    fa *= inv;
-    fb *= inv;
-  }
-  int64_t slot = 0;
-  if (cuts > 1) {  // slots: the first pieces of the blocks that are cut, then the others
-    double cut = 0.0, more = 0.0;
-    for (int i = tid; i < s; i += 256) {
-      const Blocks o = get_blocks(a, i);
-      cut += o.nb - o.past(piece);
-      more += pieces(o, piece, true);
+    mi::sync_lds();
+    const float2 ml = mlbox[(2 * qb + kp) * 32 + col];
+    const float top = fmaxf(m[0], ml.x);
+    const float fa = __builtin_amdgcn_exp2f(m[0] - top), fb = __builtin_amdgcn_exp2f(ml.x - top);
+    l[0] = l[0] * fa + ml.y * fb;
+    m[0] = top;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+#pragma unroll
+      for (int e4 = 0; e4 < 4; e4++) {
+        const f32x4 o = mine[(i * 4 + e4) * 64 + lane];
+#pragma unroll
+        for (int n = 0; n < 4; n++) acc[0][i][4 * e4 + n] = acc[0][i][4 * e4 + n] * fa + o[n] * fb;
+      }
+      asm volatile("" : "+a"(acc[0][i]));
     }
-    const int cut0 = (int)block_sum<256>(cut, sums), more0 = (int)block_sum<256>(more, sums);
-    const int b1 = q.past(piece), mine = q.nb - b1;
-    const int at = cut0 * G + h * mine + (q.nb - 1 - b);                 // of the blocks
-    const int second = more0 * G + h * (per - q.nb) + (q.nb - 1 - b);    // of the pieces k >= 1
-    if (k == 0) {
-      slot = at;
-      if (tid == 0 && at < kSplitBlocks) x.blocks[at] = int4{s, h, b, second};
+  }
+  // ---- rows to memory: 32 at a time go through LDS once more, to be written whole; what is
+  // written there is only read by its own wave.
+#pragma unroll
+  for (int c = 0; c < 2 / KP; c++) {
+    if (c) {
+      r0 += 32;
+      load_gates();
+    }
+    const float f = !whole ? 1.f : l[c] == 0.f ? 0.f : 1.f / l[c];
+#pragma unroll
+    for (int i = 0; i < 8; i++) asm volatile("" : "+a"(acc[0][i]), "+a"(acc[1][i]));  // there until used
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const bool odd = odd_row[g] < lim[c];
+#pragma unroll
+      for (int x = 0; x < 8; x++) {
+        // columns 64 g + 32 (x / 4) + 16 hl + 4 (x % 4) ..: value j is block 2 g + j / 2,
+        // element 8 (j % 2) + x; row r's piece y at y ^ (r & 7)
+        f32x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          y[j] = odd ? __builtin_nanf("") : acc[c][2 * g + (j >> 1)][8 * (j & 1) + x] * f;
+        mine[64 * col + ((16 * g + 8 * (x >> 2) + 4 * hl + (x & 3)) ^ (col & 7))] = y;
+      }
+    }
+    if (!whole) {
+      if (hl == 0 && r0 + col < nrows)
+        ((float2*)x.part_ml)[(int64_t)slot * kRows + r0 + col] = float2{m[c], l[c]};
+      for (int i = 0; i < min(32, nrows - r0); i++)
+        *(f32x4*)(x.part_o + ((int64_t)slot * kRows + r0 + i) * D + 4 * lane) = mine[64 * i + (lane ^ (i & 7))];
     } else {
-      int add = 0;
-      for (int kk = 1; kk < k; kk++) add += q.nb - q.past((int64_t)kk * piece);
-      slot = kSplitBlocks + second + add;
-    }
-    if (slot >= kSlots || (k == 0 && slot >= kSplitBlocks)) return;  // cannot be: piece_tiles
-    if (hl == 0 && r < nrows)
-      ((float2*)x.part_ml)[slot * kRows + r] = float2{top, sum};
-  }
-  // The rows go through LDS once more, to be written whole: a wave's own 32, in what it
-  // has read of the box.
+      // (the loops stay short: code that runs once a workgroup costs what its fetching does)
+      auto write = [&](int i, f32x4 y) {
+        if (r0 + i < nrows)
+          *(f16x4*)(a.out + lane64(out_at, i) + 4 * lane) =
+              f16x4{(_Float16)y[0], (_Float16)y[1], (_Float16)y[2], (_Float16)y[3]};
+      };
+      if (early) {
 #pragma unroll
-  for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 32; i++) {
+          f32x4 y = mine[64 * i + (lane ^ (i & 7))];
 #pragma unroll
-    for (int e4 = 0; e4 < 4; e4++) {
-      const f32x4 o = src[(i * 4 + e4) * 64 + lane];
+          for (int e = 0; e < 4; e++) y[e] = mi::gate_mul(y[e], (float)gates[i][e]);
+          write(i, y);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 32; i++) {
+          f32x4 y = mine[64 * i + (lane ^ (i & 7))];
+          if (a.gate) {
+            const f32x4 g = *(const f32x4*)((const float*)a.gate + lane64(gate_at, i) + 4 * lane);
 #pragma unroll
-      for (int n = 0; n < 4; n++) acc[0][i][4 * e4 + n] = acc[0][i][4 * e4 + n] * fa + o[n] * fb;
-    }
-  f32x4* const rows = box + (2 * qb + kp) * 32 * 64;  // [32][64], row r's piece x at x ^ (r & 7)
-#pragma unroll
-  for (int g = 0; g < 4; g++) {
-    const bool odd = odd_row[g] < lim[0];
-#pragma unroll
-    for (int x = 0; x < 8; x++) {
-      // columns 64 g + 32 (x / 4) + 16 hl + 4 (x % 4) ..: value j is block 2 g + j / 2,
-      // element 8 (j % 2) + x
-      f32x4 y;
-#pragma unroll
-      for (int j = 0; j < 4; j++) y[j] = odd ? __builtin_nanf("") : acc[0][2 * g + (j >> 1)][8 * (j & 1) + x];
-      rows[64 * col + ((16 * g + 8 * (x >> 2) + 4 * hl + (x & 3)) ^ (col & 7))] = y;
+            for (int e = 0; e < 4; e++) y[e] = mi::gate_mul(y[e], g[e]);
+          }
+          write(i, y);
+        }
+      }
     }
   }
-  // (Few instructions: code that runs once a workgroup costs what its fetching does.)
-  if (cuts > 1) {
-    for (int i = 0; i < min(32, nrows - r0); i++)
-      *(f32x4*)(x.part_o + (slot * kRows + r0 + i) * D + 4 * lane) = rows[64 * i + (lane ^ (i & 7))];
-    return;
   }
-  if (early) {
-#pragma unroll
-    for (int i = 0; i < 32; i++) {
-      f32x4 y = rows[64 * i + (lane ^ (i & 7))];
-      int64_t tok;
-      int head;
-      out_row(i, tok, head);
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = mi::gate_mul(y[e], (float)gates[i][e]);
-      if (r0 + i < nrows) mi::store4(a, tok, head, 4 * lane, y);
-    }
-  } else {
-    for (int i = 0; i < min(32, nrows - r0); i++) {
-      int64_t tok;
-      int head;
-      out_row(i, tok, head);
-      mi::put4(a, tok, head, 4 * lane, rows[64 * i + (lane ^ (i & 7))]);
-    }
-  }
+  if (threadIdx.x == 0) x.shares[share] = left;
 }
 
-// Joins the pieces of the blocks that are cut: a workgroup per (block, 16 rows), a
-// wave per row and four columns a thread.  A workgroup per sequence behind them
-// makes every token NaN of one beyond max_q or max_len.
+// Joins the parts of the blocks that are cut: a workgroup per (share that begins one, 16
+// rows), a wave per row and four columns a thread.  A workgroup per sequence behind
+// them makes every token NaN of one beyond max_q or max_len.
+template <int KP>
 __global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const AttnArgs a, const PrefillExtra x) {
-  if (blockIdx.x >= 8 * kSplitBlocks) {
-    const Blocks q = get_blocks(a, blockIdx.x - 8 * kSplitBlocks);
+  constexpr int kRows = rows_of(KP), kParts = kRows / 16;
+  if (blockIdx.x >= kParts * kShares) {
+    const auto q = get_blocks<KP>(a, blockIdx.x - kParts * kShares);
     const int width = a.pv.G * a.R * D;
     for (int tok = 0; tok < (q.bad ? q.nq : 0); tok++)
       for (int i = threadIdx.x; i < width; i += 256)
         a.out[(int64_t)(q.q0 + tok) * width + i] = (_Float16)__builtin_nanf("");
     return;
   }
-  const int at = blockIdx.x >> 3, part = blockIdx.x & 7;
-  const int2 c = *x.count;
-  if (at >= min(c.x, kSplitBlocks)) return;
-  const int4 blk = x.blocks[at];
-  const int s = blk.x, h = blk.y, b = blk.z, second = blk.w, piece = c.y;
-  const Blocks q = get_blocks(a, s);
+  const int share = blockIdx.x / kParts, part = blockIdx.x % kParts;
+  const Share c = x.shares[share];
+  const int next = x.shares[min(share + 1, kShares - 1)].joins;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int nrows = min(q.tb, q.nq - b * q.tb) * a.R, cuts = (q.tiles(b) + piece - 1) / piece;
-  for (int r = 16 * part + w; r < min(16 * part + 16, nrows); r += 4) {
-    float top = kNegBig, sum = 0.f;
-    f32x4 y = {};
-    int add = 0;
-    for (int k = 0; k < cuts; k++) {
-      const int64_t slot = k ? kSplitBlocks + second + add : at;
-      if (k) add += q.nb - q.past((int64_t)k * piece);
-      const float2 ml = ((const float2*)x.part_ml)[slot * kRows + r];
-      const f32x4 o = *(const f32x4*)(x.part_o + (slot * kRows + r) * D + 4 * lane);
-      const float mn = fmaxf(top, ml.x), f = __builtin_amdgcn_exp2f(top - mn),
-                  g = __builtin_amdgcn_exp2f(ml.x - mn);
-      sum = sum * f + ml.y * g;
-      y = y * f + o * g;
-      top = mn;
+  const int r0 = 16 * part + w;  // and three more, four apart
+  if (r0 >= c.rows) return;
+  int64_t gate_at[4], out_at[4];
+  f32x4 gate[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int r = min(r0 + 4 * i, c.rows - 1), tok = r / a.R, head = c.head * a.R + r - tok * a.R;
+    gate_at[i] = (int64_t)(c.token + tok) * a.g_ts + head * a.g_hs + 4 * lane;
+    out_at[i] = ((int64_t)(c.token + tok) * a.pv.G * a.R + head) * D + 4 * lane;
+  }
+  if (a.gate) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) gate[i] = mi::gate4(a, gate_at[i]);
+  }
+  float top[4], sum[4];
+  f32x4 y[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    top[i] = kNegBig;
+    sum[i] = 0.f;
+    y[i] = f32x4{};
+  }
+  for (int k = share; k <= c.last; k++) {
+    if (k > share && !(k == share + 1 ? next : x.shares[k].joins)) continue;
+    const int64_t row = (int64_t)(k > share ? 2 * k : c.slot) * kRows + r0;  // (of a slot's own)
+    float2 ml[4];
+    f32x4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      ml[i] = ((const float2*)x.part_ml)[row + 4 * i];
+      o[i] = *(const f32x4*)(x.part_o + (row + 4 * i) * D + 4 * lane);
     }
-    const int tok = r / a.R;
-    mi::put4(a, q.q0 + b * q.tb + tok, h * a.R + r - tok * a.R, 4 * lane,
-             y * (sum == 0.f ? 0.f : 1.f / sum));
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float mn = fmaxf(top[i], ml[i].x), f = __builtin_amdgcn_exp2f(top[i] - mn),
+                  g = __builtin_amdgcn_exp2f(ml[i].x - mn);
+      sum[i] = sum[i] * f + ml[i].y * g;
+      y[i] = y[i] * f + o[i] * g;
+      top[i] = mn;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (r0 + 4 * i >= c.rows) break;
+    y[i] *= sum[i] == 0.f ? 0.f : 1.f / sum[i];
+    if (a.gate)
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[i][e] = mi::gate_mul(y[i][e], gate[i][e]);
+    *(f16x4*)(a.out + out_at[i]) =
+        f16x4{(_Float16)y[i][0], (_Float16)y[i][1], (_Float16)y[i][2], (_Float16)y[i][3]};
   }
 }
 
 constexpr int kLds = 8 * kHalf + 2 * 2048;
+
+template <int KP>
+mi_status run(const AttnArgs& a, const PrefillExtra& x, hipStream_t s) {
+  static std::atomic<uint64_t> done{0};
+  MI_TRY(mi::set_lds_limit((const void*)paged_prefill_kernel<KP>, kLds, done));
+  MI_HIP(mi::launch("paged_prefill", paged_prefill_kernel<KP>, dim3(kShares), dim3(256), kLds, s, a, x));
+  MI_HIP(mi::launch("paged_merge", paged_prefill_merge_kernel<KP>,
+                    dim3((unsigned)(rows_of(KP) / 16 * kShares + a.pv.batch)), dim3(256), 0, s, a, x));
+  return MI_OK;
+}
 
 }  // namespace
 
 namespace mi {
 
 size_t paged_prefill_workspace(int32_t, int32_t, int32_t, int32_t, int, int) {
-  return (size_t)kSlots * kRows * (D + 2) * sizeof(float) + kSplitBlocks * sizeof(int4) + 64;
+  return (size_t)2 * kShares * rows_of(1) * (D + 2) * sizeof(float) + kShares * sizeof(Share);
 }
 
 mi_status paged_prefill(AttnArgs& a, void* workspace, hipStream_t s) {
-  static std::atomic<uint64_t> done{0};
-  MI_TRY(set_lds_limit((const void*)paged_prefill_kernel, kLds, done));
   PrefillExtra x;
   x.part_o = (float*)workspace;
-  x.part_ml = x.part_o + (size_t)kSlots * kRows * D;
-  x.blocks = (int4*)(x.part_ml + (size_t)kSlots * kRows * 2);
-  x.count = (int2*)(x.blocks + kSplitBlocks);
-  const int tb = kRows / a.R;
-  // blocks of the batch's sequences, and the pieces that come on top
-  const int64_t wgs = ((int64_t)a.n / tb + a.pv.batch) * a.pv.G + kShare;
-  const int64_t gx = std::min<int64_t>(wgs, 1 << 22);
-  MI_HIP(launch("paged_prefill", paged_prefill_kernel,
-                dim3((unsigned)gx, (unsigned)((wgs + gx - 1) / gx)), dim3(256), kLds, s, a, x));
-  MI_HIP(launch("paged_merge", paged_prefill_merge_kernel, dim3((unsigned)(8 * kSplitBlocks + a.pv.batch)),
-                dim3(256), 0, s, a, x));
-  return MI_OK;
+  x.part_ml = x.part_o + (size_t)2 * kShares * rows_of(1) * D;
+  x.shares = (Share*)(x.part_ml + (size_t)2 * kShares * rows_of(1) * 2);
+  // Which is faster, by the rows of the longest sequence: measured at the top.
+  return a.max_q * (int64_t)a.R > rows_of(2) ? run<1>(a, x, s) : run<2>(a, x, s);
 }
 
 }  // namespace mi
