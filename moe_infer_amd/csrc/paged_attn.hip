@@ -250,7 +250,9 @@ struct Wave {
   }
 };
 
-template <int CT>
+// SINGLE: an item to a workgroup, and nothing to join.  (A kernel of its own: with one for
+// both, the long walk was a fifth slower.)
+template <int CT, bool SINGLE>
 __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_kernel(const AttnArgs a) {
   constexpr int NW = waves(CT), NT = 64 * NW;
   extern __shared__ float lds[];
@@ -268,61 +270,88 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
   // By chunks: every item in chunks of up to kMinTiles tiles, one to a workgroup,
   // where the grid has that many.  Else a flat line of tiles, [sequence][KV
   // head][block][tile], in even pieces, one to a workgroup.
-  int s, before, f = 0, f1 = 0;
+  int s = 0, before = 0, f = 0, f1 = 0;
   const int G = a.pv.G;
   bool chunks = true;
   auto parts = [](int ntiles) { return (ntiles + kMinTiles - 1) / kMinTiles; };
-  mi::find_seq<NT>(
-      a.pv.batch,
-      [&](int i) {
-        const Seq q = get_seq<CT, false>(a, i);
-        return q.ncb * parts(q.ntiles);
-      },
-      [&](int total) {
-        chunks = (uint32_t)total * G <= (uint32_t)a.wgs;
-        f = bid;
-        f1 = min(bid + 1, total * G);
-        return chunks ? (int)((uint32_t)f / (uint32_t)G) : total;
-      },
-      s, before);
-  if (!chunks)
+  if constexpr (SINGLE) {
+    f = bid;
+    f1 = bid + 1;
+  } else {
     mi::find_seq<NT>(
         a.pv.batch,
         [&](int i) {
           const Seq q = get_seq<CT, false>(a, i);
-          return q.ncb * q.ntiles;
+          return q.ncb * parts(q.ntiles);
         },
         [&](int total) {
-          const uint32_t all = (uint32_t)total * G, each = all / a.wgs, more = all - each * a.wgs;
-          f = (int)(each * bid + min((uint32_t)bid, more));
-          f1 = f + (int)each + ((uint32_t)bid < more);
-          return (int)((uint32_t)f / (uint32_t)G);
+          chunks = (uint32_t)total * G <= (uint32_t)a.wgs;
+          f = bid;
+          f1 = min(bid + 1, total * G);
+          return chunks ? (int)((uint32_t)f / (uint32_t)G) : total;
         },
         s, before);
+    if (!chunks)
+      mi::find_seq<NT>(
+          a.pv.batch,
+          [&](int i) {
+            const Seq q = get_seq<CT, false>(a, i);
+            return q.ncb * q.ntiles;
+          },
+          [&](int total) {
+            const uint32_t all = (uint32_t)total * G, each = all / a.wgs, more = all - each * a.wgs;
+            f = (int)(each * bid + min((uint32_t)bid, more));
+            f1 = f + (int)each + ((uint32_t)bid < more);
+            return (int)((uint32_t)f / (uint32_t)G);
+          },
+          s, before);
+  }
   if (f >= f1) return;
   int slot = 2 * bid;
 
   Wave<CT> st;
   st.x16 = mi::sixteens();
   while (f < f1) {
-    const Seq sq = get_seq<CT, true>(a, s);
-    const int per = chunks ? parts(sq.ntiles) : sq.ntiles, weight = sq.ncb * per;
-    if (f >= G * (before + weight)) {
-      before += weight;
-      s++;
-      continue;
-    }
-    const uint32_t local = f - G * before, vh = local / (uint32_t)per, at = local - vh * per;
-    const int h = (int)(vh / (uint32_t)sq.ncb), cb = (int)vh - h * sq.ncb;
-    int t0, t1;
-    if (chunks) {
-      t0 = (int)(at * (uint32_t)sq.ntiles / (uint32_t)per);
-      t1 = (int)((at + 1) * (uint32_t)sq.ntiles / (uint32_t)per);
+    int h, cb, t0, t1;
+    Seq sq;
+    if constexpr (SINGLE) {
+      s = (int)((uint32_t)f / (uint32_t)(G * a.ncb));
+      const int vh = f - s * G * a.ncb;
+      h = (int)((uint32_t)vh / (uint32_t)a.ncb);
+      cb = vh - h * a.ncb;
+      sq = get_seq<CT, true>(a, s);
+      t0 = 0;
+      t1 = sq.ntiles;
       f = f1;
+      if (sq.bad) {
+        for (int i = threadIdx.x; i < (cb ? 0 : sq.nq) * a.R * D; i += NT) {
+          const int tok = i / (a.R * D);
+          a.out[((int64_t)(sq.q0 + tok) * G + h) * (a.R * D) + (i - tok * (a.R * D))] =
+              (_Float16)__builtin_nanf("");
+        }
+        return;
+      }
+      if (cb >= sq.ncb) return;
     } else {
-      t0 = (int)at;
-      t1 = min(sq.ntiles, t0 + (f1 - f));
-      f += t1 - t0;
+      sq = get_seq<CT, true>(a, s);
+      const int per = chunks ? parts(sq.ntiles) : sq.ntiles, weight = sq.ncb * per;
+      if (f >= G * (before + weight)) {
+        before += weight;
+        s++;
+        continue;
+      }
+      const uint32_t local = f - G * before, vh = local / (uint32_t)per, at = local - vh * per;
+      h = (int)(vh / (uint32_t)sq.ncb);
+      cb = (int)vh - h * sq.ncb;
+      if (chunks) {
+        t0 = (int)(at * (uint32_t)sq.ntiles / (uint32_t)per);
+        t1 = (int)((at + 1) * (uint32_t)sq.ntiles / (uint32_t)per);
+        f = f1;
+      } else {
+        t0 = (int)at;
+        t1 = min(sq.ntiles, t0 + (f1 - f));
+        f += t1 - t0;
+      }
     }
     const int c0 = cb * 16 * CT, ncols = sq.nq * a.R, first = sq.len - sq.nq;
 
@@ -448,7 +477,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       }
       __syncthreads();
     }
-    if (threadIdx.x == 0) {  // where the merge finds the item's pieces
+    if (!SINGLE && threadIdx.x == 0) {  // where the merge finds the item's pieces
       int2* const sg = a.seg + ((int64_t)s * G + h) * a.ncb + cb;
       if (whole) {
         sg->x = -1;
@@ -548,6 +577,7 @@ bool many_columns(int32_t max_q, int R) { return (int64_t)max_q * R > 32; }
 
 struct Plan {
   int ct, ncb, wgs, dsplit;
+  bool single;
   int64_t items, tiles;
   size_t o_bytes, ml_bytes, seg_bytes;
   size_t bytes() const { return o_bytes + ml_bytes + seg_bytes; }
@@ -562,6 +592,11 @@ Plan make_plan(int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
   p.tiles = p.items * (((int64_t)max_len + 31) / 32);
   const int64_t per_item = (((int64_t)max_len + 31) / 32 + kMinTiles - 1) / kMinTiles;
   p.wgs = (int)std::max<int64_t>(1, std::min<int64_t>(256, p.items * per_item));
+  // An item to a workgroup, and no merge, where that is four tiles to a wave, or more where
+  // items fill the card (one KV head's group of 8, two heads a sequence): 8 sequences of
+  // 512 rows 10.3 us against 16.5, of 1024 14.0 against 16.4, of 2048 22 against 16.5; 64 of
+  // 2048 23 against 26; 128 of 1 to 4000 42 against 68, 256 83 against 103.
+  p.single = max_len <= (p.items >= 256 ? 4096 : p.items >= 64 ? 2048 : 1024);
   p.dsplit = p.items * std::min(16 * p.ct, max_q * R) <= 256 ? 4 : 1;
   if (p.items * 16 * p.ct * p.dsplit > INT32_MAX) p.tiles = INT32_MAX;  // refused
   const int64_t cols = (int64_t)2 * p.wgs * 16 * p.ct;
@@ -571,15 +606,16 @@ Plan make_plan(int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
   return p;
 }
 
-template <int CT>
+template <int CT, bool SINGLE>
 mi_status run(AttnArgs& a, const Plan& p, hipStream_t s) {
   static std::atomic<uint64_t> done{0};
   constexpr int NW = waves(CT);
   const int fixed = (NW * 16 * (CT + 1) + 16) * (int)sizeof(float);
   const int per_col = NW * kColPitch * (int)sizeof(float);
-  MI_TRY(mi::set_lds_limit((const void*)paged_attn_kernel<CT>, fixed + 16 * per_col, done));
-  MI_HIP(mi::launch("paged_attn", paged_attn_kernel<CT>, dim3((unsigned)p.wgs), dim3(64 * NW),
-                    fixed + std::min(16, a.max_q * a.R) * per_col, s, a));
+  MI_TRY(mi::set_lds_limit((const void*)paged_attn_kernel<CT, SINGLE>, fixed + 16 * per_col, done));
+  MI_HIP(mi::launch("paged_attn", paged_attn_kernel<CT, SINGLE>, dim3((unsigned)(SINGLE ? p.items : p.wgs)),
+                    dim3(64 * NW), fixed + std::min(16, a.max_q * a.R) * per_col, s, a));
+  if (SINGLE) return MI_OK;
   const int64_t ms = p.items * 16 * CT * p.dsplit, mx = std::min<int64_t>(ms, 1 << 22);
   MI_HIP(mi::launch("paged_merge", paged_merge_kernel<CT>,
                     dim3((unsigned)mx, (unsigned)((ms + mx - 1) / mx)), dim3(256), 0, s, a));
@@ -675,5 +711,6 @@ extern "C" mi_status mi_attn_paged(
   a.dsplit = p.dsplit;
   const hipStream_t s = (hipStream_t)stream;
   if (many) return mi::paged_prefill(a, workspace, s);
-  return p.ct == 1 ? run<1>(a, p, s) : run<2>(a, p, s);
+  if (p.single) return p.ct == 1 ? run<1, true>(a, p, s) : run<2, true>(a, p, s);
+  return p.ct == 1 ? run<1, false>(a, p, s) : run<2, false>(a, p, s);
 }
