@@ -439,7 +439,7 @@ mi_status mi_attn_paged(const void* pages, int64_t num_pages, int32_t page_rows,
  * earlier records.  Kernel names: "attn_split", "attn_combine",
  * "attn_direct", "attn_prefill", "verify_wide", "kv_pack",
  * "qk_norm_rope", "matvec_bf16", "matvec_q4", "ragged_plan", "rope_apply",
- * "paged_append", "paged_read", "paged_attn", "paged_merge".
+ * "paged_append", "paged_read", "paged_attn", "paged_prefill", "paged_merge".
  * mi_prof_read returns the mean duration in microseconds and the number of
  * launches recorded since the last enable. */
 void mi_prof_enable(int on);

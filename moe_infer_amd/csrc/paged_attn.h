@@ -113,7 +113,7 @@ __device__ __forceinline__ f16x8 in_order(f16x8 x) {
 }
 
 // The prompts' form (paged_prefill.hip): workspace bytes, and the launches.
-size_t paged_prefill_workspace(int32_t batch, int32_t n, int32_t max_q, int32_t max_len, int H, int G);
+size_t paged_prefill_workspace();
 mi_status paged_prefill(AttnArgs& a, void* workspace, hipStream_t s);
 
 }  // namespace mi

@@ -14,6 +14,15 @@
 //
 // A workgroup's waves join through LDS, workgroups that share an item through
 // partials that paged_merge_kernel joins.
+//
+// Bound: for one column block, the page bytes and what a wave issues for them (64
+// sequences of up to 32768 rows, 640 MB: 132 us, 4.9 TB/s; its loads alone 121 us; a wave's
+// tile is 5300 clocks, two waves to a SIMD, of which 680 wait for memory and 13 % of the
+// walk goes to waiting at the join for the SIMD's other wave).  For two, one wave's
+// instructions (16 sequences of 4 tokens behind up to 32768 rows, 188 MB: 72 us and 5 of
+// merge; 4850 clocks a tile, 990 of them waiting).  For few tiles, the chain from the tables
+// to a page's id, its tile and the join: 8 sequences of up to 777 rows 10.3 us, one of
+// 32768 rows 12.3 and 4.9 of merge.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -569,11 +578,15 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
   mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y * (total == 0.f ? 0.f : 1.f / total));
 }
 
+// Columns that the decode kernels take at most (two blocks of 16).
+constexpr int kManyColumns = 32;
+
 // Column blocks of 16 a workgroup takes: 2 where a sequence has more than one.
 int column_blocks(int32_t max_q, int R) { return (int64_t)max_q * R <= 16 ? 1 : 2; }
 
-// Whether the prompts' form serves a call.
-bool many_columns(int32_t max_q, int R) { return (int64_t)max_q * R > 32; }
+// Whether the prompts' form serves a call: 16 sequences of 4 tokens, 8 heads a group,
+// behind 500 / 8192 / 20000 rows 20 / 55 / 80 us here and 35 / 79 / 140 there.
+bool many_columns(int32_t max_q, int R) { return (int64_t)max_q * R > kManyColumns; }
 
 struct Plan {
   int ct, ncb, wgs, dsplit;
@@ -604,6 +617,13 @@ Plan make_plan(int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
   p.ml_bytes = cols * 2 * sizeof(float);
   p.seg_bytes = (p.items * sizeof(int2) + 15) & ~(size_t)15;
   return p;
+}
+
+// A prompt's workspace also serves the smaller calls that the decode kernels take.
+size_t plan_bytes(const Plan& p, int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
+  if (!many_columns(max_q, H / G)) return p.bytes();
+  const Plan few = make_plan(batch, std::max(1, kManyColumns / (H / G)), max_len, H, G);
+  return std::max(mi::paged_prefill_workspace(), few.bytes());
 }
 
 template <int CT, bool SINGLE>
@@ -643,9 +663,7 @@ extern "C" size_t mi_attn_paged_workspace_size(int32_t batch, int32_t n, int32_t
   max_q = std::min(max_q, n);
   const Plan p = make_plan(batch, max_q, max_len, num_q_heads, num_kv_heads);
   if (p.tiles >= INT32_MAX) return 0;
-  return many_columns(max_q, num_q_heads / num_kv_heads)
-             ? mi::paged_prefill_workspace(batch, n, max_q, max_len, num_q_heads, num_kv_heads)
-             : p.bytes();
+  return plan_bytes(p, batch, max_q, max_len, num_q_heads, num_kv_heads);
 }
 
 extern "C" mi_status mi_attn_paged(
@@ -686,9 +704,7 @@ extern "C" mi_status mi_attn_paged(
     return mi::fail(MI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d rows in one call", batch, max_q,
                     max_len);
   const bool many = many_columns(max_q, num_q_heads / num_kv_heads);
-  const size_t need = many ? mi::paged_prefill_workspace(batch, n, max_q, max_len, num_q_heads,
-                                                         num_kv_heads)
-                           : p.bytes();
+  const size_t need = plan_bytes(p, batch, max_q, max_len, num_q_heads, num_kv_heads);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return mi::fail(MI_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, need);
   a.q = (const _Float16*)q;

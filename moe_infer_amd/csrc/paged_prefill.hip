@@ -26,7 +26,6 @@
 // begins and another ends, the merge kernel joins: it reads and writes as much as the
 // partials are, 28 us for 128 blocks of 256 rows.
 #include <algorithm>
-#include <cmath>
 
 #include "paged_attn.h"
 
@@ -678,12 +677,14 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   if (threadIdx.x == 0) x.shares[share] = left;
 }
 
-// Joins the parts of the blocks that are cut: a workgroup per (share that begins one, 16
-// rows), a wave per row and four columns a thread.  A workgroup per sequence behind
-// them makes every token NaN of one beyond max_q or max_len.
+// Joins the parts of the blocks that are cut: a workgroup per (share that begins one, 8
+// rows), four columns a thread; wave w takes four of the rows and every other part from
+// w / 2 on, and two waves join through LDS.  A workgroup per sequence behind them makes
+// every token NaN of one beyond max_q or max_len.
+constexpr int kMergeRows = 8;
 template <int KP>
 __global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const AttnArgs a, const PrefillExtra x) {
-  constexpr int kRows = rows_of(KP), kParts = kRows / 16;
+  constexpr int kRows = rows_of(KP), kParts = kRows / kMergeRows;
   if (blockIdx.x >= kParts * kShares) {
     const auto q = get_blocks<KP>(a, blockIdx.x - kParts * kShares);
     const int width = a.pv.G * a.R * D;
@@ -692,23 +693,21 @@ __global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const AttnArgs
         a.out[(int64_t)(q.q0 + tok) * width + i] = (_Float16)__builtin_nanf("");
     return;
   }
+  __shared__ f32x4 box[2][4][64];
+  __shared__ float2 mlbox[2][4];
   const int share = blockIdx.x / kParts, part = blockIdx.x % kParts;
   const Share c = x.shares[share];
-  const int next = x.shares[min(share + 1, kShares - 1)].joins;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int r0 = 16 * part + w;  // and three more, four apart
-  if (r0 >= c.rows) return;
-  int64_t gate_at[4], out_at[4];
-  f32x4 gate[4];
+  if (kMergeRows * part >= c.rows) return;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r0 = kMergeRows * part + 4 * (w & 1), half = w >> 1;
+  // the two rows that the wave writes, and their gates
+  int64_t out_at[2];
+  f32x4 gate[2];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const int r = min(r0 + 4 * i, c.rows - 1), tok = r / a.R, head = c.head * a.R + r - tok * a.R;
-    gate_at[i] = (int64_t)(c.token + tok) * a.g_ts + head * a.g_hs + 4 * lane;
+  for (int i = 0; i < 2; i++) {
+    const int r = min(r0 + 2 * half + i, c.rows - 1), tok = r / a.R, head = c.head * a.R + r - tok * a.R;
     out_at[i] = ((int64_t)(c.token + tok) * a.pv.G * a.R + head) * D + 4 * lane;
-  }
-  if (a.gate) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) gate[i] = mi::gate4(a, gate_at[i]);
+    if (a.gate) gate[i] = mi::gate4(a, (int64_t)(c.token + tok) * a.g_ts + head * a.g_hs + 4 * lane);
   }
   float top[4], sum[4];
   f32x4 y[4];
@@ -718,34 +717,54 @@ __global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const AttnArgs
     sum[i] = 0.f;
     y[i] = f32x4{};
   }
-  for (int k = share; k <= c.last; k++) {
-    if (k > share && !(k == share + 1 ? next : x.shares[k].joins)) continue;
-    const int64_t row = (int64_t)(k > share ? 2 * k : c.slot) * kRows + r0;  // (of a slot's own)
-    float2 ml[4];
-    f32x4 o[4];
+  // Two parts at a time; what is not one weighs nothing, in the place of the first.
+  for (int k0 = share + half; k0 <= c.last; k0 += 4) {
+    float2 ml[2][4];
+    f32x4 o[2][4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      ml[i] = ((const float2*)x.part_ml)[row + 4 * i];
-      o[i] = *(const f32x4*)(x.part_o + (row + 4 * i) * D + 4 * lane);
+    for (int u = 0; u < 2; u++) {
+      const int k = min(k0 + 2 * u, kShares - 1);
+      const bool in = k == share || (k0 + 2 * u <= c.last && x.shares[k].joins);
+      const int64_t row = (int64_t)(in && k > share ? 2 * k : c.slot) * kRows + r0;  // (of a slot's own)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        ml[u][i] = ((const float2*)x.part_ml)[row + i];
+        o[u][i] = *(const f32x4*)(x.part_o + (row + i) * D + 4 * lane);
+        if (!in) ml[u][i] = float2{kNegBig, 0.f};
+      }
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const float mn = fmaxf(top[i], ml[i].x), f = __builtin_amdgcn_exp2f(top[i] - mn),
-                  g = __builtin_amdgcn_exp2f(ml[i].x - mn);
-      sum[i] = sum[i] * f + ml[i].y * g;
-      y[i] = y[i] * f + o[i] * g;
+      const float mn = fmaxf(top[i], fmaxf(ml[0][i].x, ml[1][i].x));
+      const float f = __builtin_amdgcn_exp2f(top[i] - mn), g0 = __builtin_amdgcn_exp2f(ml[0][i].x - mn),
+                  g1 = __builtin_amdgcn_exp2f(ml[1][i].x - mn);
+      sum[i] = sum[i] * f + ml[0][i].y * g0 + ml[1][i].y * g1;
+      y[i] = y[i] * f + o[0][i] * g0 + o[1][i] * g1;
       top[i] = mn;
     }
   }
+  // wave (w & 1, half) hands rows 2 (1 - half) .. of its four to the other half's
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (r0 + 4 * i >= c.rows) break;
-    y[i] *= sum[i] == 0.f ? 0.f : 1.f / sum[i];
+  for (int i = 0; i < 2; i++) {
+    const int j = 2 * (1 - half) + i;
+    const f32x4 mine = half ? y[i] : y[2 + i];
+    box[w & 1][j][lane] = mine;
+    if (lane == 0) mlbox[w & 1][j] = half ? float2{top[i], sum[i]} : float2{top[2 + i], sum[2 + i]};
+  }
+  mi::sync_lds();
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int j = 2 * half + i;
+    if (r0 + j >= c.rows) break;
+    const float2 ml = mlbox[w & 1][j];
+    const float t = half ? top[2 + i] : top[i], l = half ? sum[2 + i] : sum[i], mn = fmaxf(t, ml.x);
+    const float f = __builtin_amdgcn_exp2f(t - mn), g = __builtin_amdgcn_exp2f(ml.x - mn);
+    const float all = l * f + ml.y * g, inv = all == 0.f ? 0.f : 1.f / all;
+    f32x4 z = ((half ? y[2 + i] : y[i]) * f + box[w & 1][j][lane] * g) * inv;
     if (a.gate)
 #pragma unroll
-      for (int e = 0; e < 4; e++) y[i][e] = mi::gate_mul(y[i][e], gate[i][e]);
-    *(f16x4*)(a.out + out_at[i]) =
-        f16x4{(_Float16)y[i][0], (_Float16)y[i][1], (_Float16)y[i][2], (_Float16)y[i][3]};
+      for (int e = 0; e < 4; e++) z[e] = mi::gate_mul(z[e], gate[i][e]);
+    *(f16x4*)(a.out + out_at[i]) = f16x4{(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]};
   }
 }
 
@@ -757,7 +776,7 @@ mi_status run(const AttnArgs& a, const PrefillExtra& x, hipStream_t s) {
   MI_TRY(mi::set_lds_limit((const void*)paged_prefill_kernel<KP>, kLds, done));
   MI_HIP(mi::launch("paged_prefill", paged_prefill_kernel<KP>, dim3(kShares), dim3(256), kLds, s, a, x));
   MI_HIP(mi::launch("paged_merge", paged_prefill_merge_kernel<KP>,
-                    dim3((unsigned)(rows_of(KP) / 16 * kShares + a.pv.batch)), dim3(256), 0, s, a, x));
+                    dim3((unsigned)(rows_of(KP) / kMergeRows * kShares + a.pv.batch)), dim3(256), 0, s, a, x));
   return MI_OK;
 }
 
@@ -765,7 +784,7 @@ mi_status run(const AttnArgs& a, const PrefillExtra& x, hipStream_t s) {
 
 namespace mi {
 
-size_t paged_prefill_workspace(int32_t, int32_t, int32_t, int32_t, int, int) {
+size_t paged_prefill_workspace() {
   return (size_t)2 * kShares * rows_of(1) * (D + 2) * sizeof(float) + kShares * sizeof(Share);
 }
 
