@@ -585,7 +585,7 @@ constexpr int kManyColumns = 32;
 int column_blocks(int32_t max_q, int R) { return (int64_t)max_q * R <= 16 ? 1 : 2; }
 
 // Whether the prompts' form serves a call: 16 sequences of 4 tokens, 8 heads a group,
-// behind 500 / 8192 / 20000 rows 20 / 55 / 80 us here and 35 / 79 / 140 there.
+// behind 500 / 8192 / 20000 rows 20 / 56 / 81 us here and 34 / 72 / 136 there.
 bool many_columns(int32_t max_q, int R) { return (int64_t)max_q * R > kManyColumns; }
 
 struct Plan {
@@ -662,7 +662,7 @@ extern "C" size_t mi_attn_paged_workspace_size(int32_t batch, int32_t n, int32_t
     return 0;
   max_q = std::min(max_q, n);
   const Plan p = make_plan(batch, max_q, max_len, num_q_heads, num_kv_heads);
-  if (p.tiles >= INT32_MAX) return 0;
+  if (p.tiles >= INT32_MAX && !many_columns(max_q, num_q_heads / num_kv_heads)) return 0;
   return plan_bytes(p, batch, max_q, max_len, num_q_heads, num_kv_heads);
 }
 
@@ -700,10 +700,10 @@ extern "C" mi_status mi_attn_paged(
   }
   max_q = std::min(max_q, n);
   const Plan p = make_plan(batch, max_q, max_len, num_q_heads, num_kv_heads);
-  if (p.tiles >= INT32_MAX)
+  const bool many = many_columns(max_q, num_q_heads / num_kv_heads);
+  if (p.tiles >= INT32_MAX && !many)  // the decode kernels count them in 32 bits
     return mi::fail(MI_ERR_UNSUPPORTED, "%d sequences of %d tokens and %d rows in one call", batch, max_q,
                     max_len);
-  const bool many = many_columns(max_q, num_q_heads / num_kv_heads);
   const size_t need = plan_bytes(p, batch, max_q, max_len, num_q_heads, num_kv_heads);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)
     return mi::fail(MI_ERR_INVALID_ARG, "workspace of %zu bytes, %zu needed", workspace_bytes, need);

@@ -9,8 +9,8 @@
 // from LDS feeds two products.  KP = 1: four waves use what is dequantised, 3600 clocks
 // a tile to a wave, 2048 of them MFMA; KP = 2: two do, 4600 clocks, and the two halves of
 // the keys join at the end, but a block is half as long, which is what a sequence of up
-// to 128 rows wants (16 of 128 rows behind 8192: 82 us against 95; 16 of 160: 120
-// against 97; a prompt of 4096 tokens, 512 rows a KV head and 64 tokens: 209 against 197).
+// to 128 rows wants (16 sequences of 128 rows behind 8192: 75 us against 88 for KP = 1; 16 of
+// 160: 113 against 90; a prompt of 4096 tokens, 8 heads a group: 232 against 194).
 //
 // Bound: the instructions that a wave alone on its SIMD issues (535 of four clocks a tile
 // for KP = 1 and 690 for KP = 2, 64 of them MFMAs of 32 clocks).  What a tile needs besides
@@ -24,7 +24,7 @@
 // workgroup a CU: ragged batches and causal prompts cost what they hold (chunks behind
 // 2000 to 16000 rows: 366 us against 430 where whole pieces were dealt).  What a share
 // begins and another ends, the merge kernel joins: it reads and writes as much as the
-// partials are, 28 us for 128 blocks of 256 rows.
+// partials are, 22 us for 128 blocks of 256 rows.
 #include <algorithm>
 
 #include "paged_attn.h"
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   for (int i = 0; i < 4; i++) id[i] = ids(ta + i);
   idn = ids(ta + 4);
   const float rinv = 1.f / (float)a.R;
-  auto token = [&](int r) { return (int)(((float)r + 0.5f) * rinv); };  // r / R: r < 128
+  auto token = [&](int r) { return (int)(((float)r + 0.5f) * rinv); };  // r / R: r < 256
   {
     f16x8 y[kRows / 8];
 #pragma unroll

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import moe_infer_amd as m
+from moe_infer_amd.paged import TILE_BYTES
 
 from . import paged_ref as R
 from .gpu_util import announce
@@ -170,3 +171,38 @@ def test_captured_prompts_share_a_workspace():
         for q, new, o in ((q1, long, o1), (q2, short, o2)):
             ref, limit = pool.reference(q, new)
             near(o, ref, limit, f"replay {i}")
+
+
+def test_prompts_of_pages_past_32_bits():
+    """Both forms over a pool of more than 4 GiB whose last pages they read."""
+    per = 2 * 2 * TILE_BYTES
+    num = (1 << 32) // per + 40
+    pages = torch.empty((num, 2, 2, TILE_BYTES), dtype=torch.uint8, device="cuda")
+    pool = Pool(17, [150], spare=0)
+    table = np.array([[num - 1, num - 5, num - 2]], np.int32)
+    for j in range(3):
+        pages[table[0, j]] = pool.pages[pool.table[0, j]]
+    for n in (10, 60):
+        q = randn(gen(18 + n), n, 16, D)
+        want = m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of([n]), q, n, 150)
+        assert torch.equal(m.attn_prefill_paged(pages, i32(table), pool.len, cu_of([n]), q, n, 150), want)
+    del pages
+
+
+def test_two_prompts_at_once():
+    """Calls on two streams, each with its own workspace, over the same pages."""
+    pool = Pool(19, [3000, 2500])
+    new = [90, 33]
+    cu, g = cu_of(new), gen(20)
+    qs = [randn(g, sum(new), 16, D) for _ in range(2)]
+    want = [m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu, q, 90, 3000) for q in qs]
+    ws = [m.paged_workspace(2, sum(new), 90, 3000) for _ in range(2)]
+    out = [torch.empty_like(q) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s, q, o, w in zip(streams, qs, out, ws):
+            with torch.cuda.stream(s):
+                m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu, q, 90, 3000, out=o, workspace=w)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
