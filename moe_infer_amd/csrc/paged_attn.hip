@@ -382,13 +382,14 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
     const int tm = max(t0, min(t1, lim0 >> 5));
 
     st.clear();
-    // A page that is not there is read as no bytes and the sums become not a number.
+    // A page that is not there is read as no bytes and the sums of the columns that see it
+    // become not a number.
     // kAhead tiles are under way, in turn; pages are looked up another one ahead.
     constexpr int kAhead = ahead(CT);
-    bool lost = false;
+    int lost = INT32_MAX;  // least row in sight whose page is not there
     auto buffer = [&](int32_t id, int t) {
       const uint8_t* p = t < t1 ? a.pv.at(id, h, t) : nullptr;
-      lost = lost || (t < t1 && !p);
+      if (t < t1 && !p) lost = min(lost, 32 * t);
       return Tile::buffer(p);
     };
     auto page = [&](int t) { return t < t1 ? a.pv.page(s, t) : -1; };
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
       st.l[ct] = mi::sum_rows(st.l[ct]);
-      if (lost) st.l[ct] = __builtin_nanf("");
+      if (lost < st.lim[ct]) st.l[ct] = __builtin_nanf("");
       if (lane < 16) mbox[(w * CT + ct) * 16 + lane] = st.m[ct];
     }
     // from here on the lane's addresses are formed anew: hoisted out of the loop

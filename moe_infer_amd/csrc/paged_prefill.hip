@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
   // registers every thread would hold 20 words of them).
   u32x4 rk[KP], rv[KP];
   uint32_t sk, sv;
-  bool lost = false;
+  int lost = INT32_MAX;  // least row in sight whose page is not there
   // Where tiles t + 1, t + 2 and t + 3 lie (at[i][u]: 32-row tile KP (t + i) + u), looked up a tile
   // before their loads; the page's id is loaded two tiles before that, by a vector load
   // (a scalar one would hold up every wait for LDS until it has come).  What has no
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
     for (int u = 0; u < KP; u++) {
       const uint32_t id = __builtin_amdgcn_readlane(idv, u);
       const int ok = (KP * t + u < tlim) & (id < npages);
-      lost = lost | ((KP * t + u < tend) & (ok ^ 1));
+      if ((KP * t + u < tend) & (ok ^ 1)) lost = min(lost, 32 * (KP * t + u));
       const uint64_t off = id * page_bytes + (uint32_t)(((KP * t + u) & ((1 << pt) - 1)) * mi::kTileBytes);
       p[u] = pages + (ok ? off : 0);
     }
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
 #pragma unroll
   for (int c = 0; c < 2; c++) {
     l[c] = mi::sum_xor32(l[c]);
-    if (lost) l[c] = __builtin_nanf("");
+    if (lost < lim[c]) l[c] = __builtin_nanf("");
   }
   __syncthreads();  // every wave is done with the tiles
 

@@ -206,3 +206,22 @@ def test_two_prompts_at_once():
                 m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu, q, 90, 3000, out=o, workspace=w)
     torch.cuda.synchronize()
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize("new,past", [(3, 62), (16, 56), (20, 50), (100, 40), (100, 3000)])
+def test_a_lost_page_is_lost_to_those_that_see_it(new, past):
+    """Every form: the tokens before the first row of a page that is not there are whole."""
+    lens = [new + past, 70]
+    pool = Pool(21, lens, page_rows=32)
+    q = randn(gen(22), new + 2, 16, D)
+    cu = cu_of([new, 2])
+    ref, limit = pool.reference(q, [new, 2])
+    gone = (past // 32 + 1) * 32  # a page's first row, within the new ones
+    assert past < gone < new + past
+    pool.table[0, gone // 32] = -1
+    for bound in (max(lens), 9000):
+        out = f64(m.attn_prefill_paged(pool.pages, i32(pool.table), pool.len, cu, q, new, bound))
+        seen = gone - past
+        near(out[:seen], ref[:seen], limit[:seen], "before it")
+        assert np.all(np.isnan(out[seen:new]))
+        near(out[new:], ref[new:], limit[new:], "the other sequence")
