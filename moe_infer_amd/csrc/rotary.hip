@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(256) rope_apply_kernel(const RopeApplyArgs a) 
     float y[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
     if (a.norm_w) mi::rms_norm<float>(y, a.norm_w, a.eps, lane);
     t.apply(a.plan, y, lane);
-    mi::store4((TO*)a.out + (tok * a.heads + h0 + i) * mi::kHeadDim + 4 * lane, y);
+    mi::store4<EACH != 1>((TO*)a.out + (tok * a.heads + h0 + i) * mi::kHeadDim + 4 * lane, y);
   }
 }
 
