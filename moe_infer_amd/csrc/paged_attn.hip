@@ -16,7 +16,7 @@
 // partials that paged_merge_kernel joins.
 //
 // Bound: for one column block, the page bytes and what a wave issues for them (64
-// sequences of up to 32768 rows, 640 MB: 132 us, 4.9 TB/s; its loads alone 121 us; a wave's
+// sequences of up to 32768 rows, 640 MB: 126.5 us, 5.1 TB/s; a wave's
 // tile is 5300 clocks, two waves to a SIMD, of which 680 wait for memory and 13 % of the
 // walk goes to waiting at the join for the SIMD's other wave).  For two, one wave's
 // instructions (16 sequences of 4 tokens behind up to 32768 rows, 188 MB: 72 us and 5 of
@@ -78,8 +78,10 @@ struct Tile {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, p ? mi::kTileBytes : 0,
                                              0x00020000);
   }
+  // (Past the caches, bit 1: a call reads a page's bytes once.  64 sequences 126.5 us, 133.7
+  // without; the same for the small ones.)
   static __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t b, int lane_at, int at) {
-    return __builtin_amdgcn_raw_buffer_load_b128(b, lane_at + at, 0, 0);
+    return __builtin_amdgcn_raw_buffer_load_b128(b, lane_at + at, 0, 2);
   }
   __device__ __forceinline__ void load_k(__amdgpu_buffer_rsrc_t b, int lane) {
 #pragma unroll
