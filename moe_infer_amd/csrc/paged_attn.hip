@@ -335,11 +335,10 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       t1 = sq.ntiles;
       f = f1;
       if (sq.bad) {
-        for (int i = threadIdx.x; i < (cb ? 0 : sq.nq) * a.R * D; i += NT) {
-          const int tok = i / (a.R * D);
-          a.out[((int64_t)(sq.q0 + tok) * G + h) * (a.R * D) + (i - tok * (a.R * D))] =
-              (_Float16)__builtin_nanf("");
-        }
+        const int width = a.R * D;
+        for (int tok = 0; tok < (cb ? 0 : sq.nq); tok++)
+          for (int i = threadIdx.x; i < width; i += NT)
+            a.out[((int64_t)(sq.q0 + tok) * G + h) * width + i] = (_Float16)__builtin_nanf("");
         return;
       }
       if (cb >= sq.ncb) return;

@@ -329,7 +329,9 @@ def paged_read(pages: torch.Tensor, block_table: torch.Tensor, kv_len: torch.Ten
 def paged_workspace(batch: int, n: int, max_q: int, max_len: int, num_q_heads: int = 16,
                     num_kv_heads: int = 2, device="cuda") -> torch.Tensor:
     """Workspace of attn_decode_paged / attn_prefill_paged for steps of these
-    sizes (n tokens in all, at most max_q and max_len rows a sequence)."""
+    sizes (n tokens in all, at most max_q and max_len rows a sequence) and smaller
+    ones; 135 MB where a sequence brings more than 32 tokens times heads of a group.
+    Calls that may run at the same time need one each."""
     nbytes = _lib.lib().mi_attn_paged_workspace_size(batch, n, max_q, max_len, num_q_heads,
                                                      num_kv_heads)
     if not nbytes:
@@ -380,7 +382,8 @@ def attn_prefill_paged(pages: torch.Tensor, block_table: torch.Tensor, kv_len: t
     """Causal attention of a ragged batch, its rows already appended: q [n, H, 256]
     f16, tokens cu_q[s] .. cu_q[s + 1] - 1 the last rows of sequence s (at most
     max_q tokens and max_len rows).  Prompts, chunks behind cached rows, drafts to
-    verify.  gate and out as for attn_decode_paged."""
+    verify.  gate and out as for attn_decode_paged; tokens from cu_q[-1] on are not
+    written."""
     if cu_q is None:
         raise TypeError("cu_q must be a torch.Tensor")
     return _attend(pages, block_table, kv_len, cu_q, q, int(max_q), int(max_len), gate, out, workspace)
