@@ -8,8 +8,8 @@
 // it (v_mfma_f32_32x32x16_f16, S^T = K Q^T, O^T += V^T P^T), so that every operand read
 // from LDS feeds two products.  KP = 1: four waves use what is dequantised, 3600 clocks
 // a tile to a wave, 2048 of them MFMA; KP = 2: two do, 4600 clocks, and the two halves of
-// the keys join at the end, but a block is half as long, which is what a sequence of up
-// to 128 rows wants (16 sequences of 128 rows behind 8192: 75 us against 88 for KP = 1; 16 of
+// the keys join at the end, but a block is half as long, which is what small calls and
+// sequences of up to 128 rows want (16 sequences of 128 rows behind 8192: 75 us against 88 for KP = 1; 16 of
 // 160: 113 against 90; a prompt of 4096 tokens, 8 heads a group: 232 against 194).
 //
 // Bound: the instructions that a wave alone on its SIMD issues (535 of four clocks a tile
@@ -793,8 +793,11 @@ mi_status paged_prefill(AttnArgs& a, void* workspace, hipStream_t s) {
   x.part_o = (float*)workspace;
   x.part_ml = x.part_o + (size_t)2 * kShares * rows_of(1) * D;
   x.shares = (Share*)(x.part_ml + (size_t)2 * kShares * rows_of(1) * 2);
-  // Which is faster, by the rows of the longest sequence: measured at the top.
-  return a.max_q * (int64_t)a.R > rows_of(2) ? run<1>(a, x, s) : run<2>(a, x, s);
+  // Short blocks for sequences of up to 128 rows (measured at the top) and for calls too
+  // small to fill the card, by rows times the longest sequence (at 2.6 M 35 us against
+  // 43.5, at 5.1 M 38 and 44, at 17.9 M 54 and 56.5; at 32 M 84 and 75, at 67 M 92 and 77).
+  const bool few = (double)a.n * a.R * a.pv.G * a.max_len < 20e6;
+  return few || a.max_q * (int64_t)a.R <= rows_of(2) ? run<2>(a, x, s) : run<1>(a, x, s);
 }
 
 }  // namespace mi

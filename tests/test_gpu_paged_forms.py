@@ -68,7 +68,8 @@ def test_prompt_forms(H, G, rows, past):
     g = gen(7)
     q, gate = randn(g, sum(new), H, D), randn(g, sum(new), H, D)
     ref, limit = pool.reference(q, new)
-    near(m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(new), q, max(new), max(lens)), ref, limit, "no gate")
+    for bound in (max(lens), 1 << 24):  # the size of a call goes by its bounds
+        near(m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(new), q, max(new), bound), ref, limit, "no gate")
     for gt in (gate, gate.float()):
         ref, limit = pool.reference(q, new, gt)
         out = m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(new), q, max(new), max(lens), gate=gt)
@@ -86,8 +87,9 @@ def test_prompts_of_many_sequences():
     pool = Pool(9, lens, G=1, page_rows=32)
     q = randn(gen(10), sum(new), 8, D)
     ref, limit = pool.reference(q, new)
-    out = m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(new), q, 40, max(lens))
-    near(out, ref, limit, "330 sequences")
+    for bound in (max(lens), 1 << 24):
+        out = m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(new), q, 40, bound)
+        near(out, ref, limit, f"330 sequences, bound {bound}")
 
 
 def test_prompts_beside_what_is_refused():
@@ -219,9 +221,40 @@ def test_a_lost_page_is_lost_to_those_that_see_it(new, past):
     gone = (past // 32 + 1) * 32  # a page's first row, within the new ones
     assert past < gone < new + past
     pool.table[0, gone // 32] = -1
-    for bound in (max(lens), 9000):
+    for bound in (max(lens), 1 << 24):
         out = f64(m.attn_prefill_paged(pool.pages, i32(pool.table), pool.len, cu, q, new, bound))
         seen = gone - past
         near(out[:seen], ref[:seen], limit[:seen], "before it")
         assert np.all(np.isnan(out[seen:new]))
         near(out[new:], ref[new:], limit[new:], "the other sequence")
+
+
+@pytest.mark.parametrize("H,G", [(16, 2), (9, 3)])
+def test_prompts_of_long_blocks(H, G):
+    """Calls that fill the card: blocks of 256 rows, cut and whole, every kind of row in
+    them."""
+    new, past = [530, 3, 257, 0, 64], [1500, 700, 0, 30, 2]
+    lens = [a + b for a, b in zip(new, past)]
+    pool = Pool(23, lens, G=G, page_rows=32)
+    poison_tail(pool, lens)
+    g = gen(24)
+    q, gate = randn(g, sum(new), H, D), randn(g, sum(new), H, D)
+    ref, limit = pool.reference(q, new, gate)
+    for gt in (gate, gate.float()):
+        for bound in (max(lens), 9000):
+            out = m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(new), q, max(new), bound, gate=gt)
+            near(out, ref, limit, f"bound {bound}")
+    # a NaN scale of V in a row that only the later tokens of a block see, and a lost page
+    h = pool.host.view(np.float16)
+    row = 1600
+    h[pool.table[0, row // 32], 0, 0, R.V_SO[row % 32][64]] = np.nan
+    pool.put()
+    pool.table[0, 1856 // 32] = -1
+    out = f64(m.attn_prefill_paged(pool.pages, i32(pool.table), pool.len, cu_of(new), q, max(new), 9000, gate=gate))
+    ratio = H // G
+    near(out[:100], ref[:100], limit[:100], "before both")
+    near(out[:356, ratio:], ref[:356, ratio:], limit[:356, ratio:], "the other KV heads before the page")
+    assert np.all(np.isnan(out[100:356, :ratio, 64:128])) and np.all(np.isnan(out[356:530]))
+    rest = np.r_[0:64, 128:256]
+    near(out[100:356, :ratio][..., rest], ref[100:356, :ratio][..., rest], limit[100:356, :ratio][..., rest], "other groups")
+    near(out[530:], ref[530:], limit[530:], "the other sequences")
