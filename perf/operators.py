@@ -155,12 +155,6 @@ def _frequencies(rot, scaling):
     return f, 0.1 * math.log(s) + 1.0 if scaling == "yarn" else 1.0
 
 
-def _scaling_argument(scaling):
-    if scaling == "none":
-        return None
-    return {"type": scaling, "factor": 4.0, **({"original_max_position": 8192} if scaling == "yarn" else {})}
-
-
 def _tables(gen, rows, page):
     """A pool of pages in no order: (pages in the pool, block table, unused entries -1)."""
     need = [-(-r // page) for r in rows]
@@ -248,8 +242,11 @@ def _keep(s, name, make):
 
 def _own_rope(m, s):
     c = s["case"]
-    return _keep(s, "rope", lambda: m.Rope(rotary_dim=c["rot"], theta=1e7, layout=c["layout"],
-                                           scaling=_scaling_argument(c["scaling"])))
+    if c["scaling"] == "yarn":  # the ramp is this file's, by turns, not what a type's name stands for
+        f, factor = _frequencies(c["rot"], "yarn")
+        return _keep(s, "rope", lambda: m.Rope(rotary_dim=c["rot"], layout=c["layout"], frequencies=f, factor=factor))
+    scaling = None if c["scaling"] == "none" else {"type": c["scaling"], "factor": 4.0}
+    return _keep(s, "rope", lambda: m.Rope(rotary_dim=c["rot"], theta=1e7, layout=c["layout"], scaling=scaling))
 
 
 def _run_own(s):
