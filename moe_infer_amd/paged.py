@@ -48,10 +48,13 @@ class Rope:
     "type" and "factor" s (>= 1), stretches it for a context s times longer:
       "linear"  every frequency / s
       "ntk"     theta * s^(rotary_dim / (rotary_dim - 2)) in theta's place
-      "yarn"    by the turns r a pair makes over "original_max_position" rows:
-                frequency * (g + (1 - g) / s), g = (r - beta_slow) / (beta_fast - beta_slow)
-                held to [0, 1] ("beta_slow" 1, "beta_fast" 32), and the rotated columns
-                times "attention_factor" (default 0.1 ln s + 1)
+      "yarn"    frequency i * (1 - g + g / s), g = (i - first) / (last - first) held to
+                [0, 1], first and last the pairs that make "beta_fast" (32) and "beta_slow"
+                (1) turns r over "original_max_position" rows L,
+                rotary_dim ln(L / (2 pi r)) / (2 ln theta), rounded down and up: what a
+                config.json means; and the rotated columns times "attention_factor"
+                (default 0.1 ln s + 1).  "ramp": "turns" instead of "pairs": a line in
+                the turns, g = (beta_fast - r) / (beta_fast - beta_slow)
     frequencies: a sequence of rotary_dim / 2 numbers instead of all that."""
 
     def __init__(self, rotary_dim: int = 64, theta: float = 1e7, layout: str = "half",
@@ -108,7 +111,7 @@ def _scaled(dim: int, theta: float, scaling: dict):
             raise ValueError(f"scaling has no type but {sorted(scaling)}")
         return [theta ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0
     known = {"linear": set(), "ntk": set(),
-             "yarn": {"original_max_position", "beta_fast", "beta_slow", "attention_factor"}}
+             "yarn": {"original_max_position", "beta_fast", "beta_slow", "ramp", "attention_factor"}}
     if kind not in known:
         raise ValueError(f"scaling type {kind!r}: one of {sorted(known)}")
     if "factor" not in scaling:
@@ -129,11 +132,21 @@ def _scaled(dim: int, theta: float, scaling: dict):
         raise ValueError("yarn needs original_max_position")
     rows = float(scaling["original_max_position"])
     slow, fast = float(scaling.get("beta_slow", 1.0)), float(scaling.get("beta_fast", 32.0))
-    if not (rows > 0 and fast > slow):
-        raise ValueError(f"yarn: original_max_position {rows}, beta_slow {slow}, beta_fast {fast}")
-    keep = [min(1.0, max(0.0, (rows * x / (2 * math.pi) - slow) / (fast - slow))) for x in f]
+    ramp = scaling.get("ramp", "pairs")
+    if not (rows > 0 and fast > slow) or (ramp == "pairs" and not (slow > 0 and theta > 1)):
+        raise ValueError(f"yarn: original_max_position {rows}, beta_slow {slow}, beta_fast {fast}, theta {theta}")
+    if ramp == "turns":
+        share = [(fast - rows * x / (2 * math.pi)) / (fast - slow) for x in f]
+    elif ramp == "pairs":
+        pair = [dim * math.log(rows / (2 * math.pi * r)) / (2 * math.log(theta)) for r in (fast, slow)]
+        first, last = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), dim - 1)
+        if first > last and dim:
+            raise ValueError(f"yarn: no pair of {dim} columns makes {slow} to {fast} turns in {rows} rows")
+        share = [(i - first) / max(last - first, 0.001) for i in range(dim // 2)]
+    else:
+        raise ValueError(f"yarn: ramp {ramp!r}: 'pairs' or 'turns'")
     factor = scaling.get("attention_factor")
-    return ([x * (g + (1.0 - g) / s) for x, g in zip(f, keep)],
+    return ([x * (1.0 - g + g / s) for x, g in zip(f, (min(1.0, max(0.0, g)) for g in share))],
             0.1 * math.log(s) + 1.0 if factor is None else float(factor))
 
 
