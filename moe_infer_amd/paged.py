@@ -51,8 +51,8 @@ class Rope:
       "yarn"    frequency i * (1 - g + g / s), g = (i - first) / (last - first) held to
                 [0, 1], first and last the pairs that make "beta_fast" (32) and "beta_slow"
                 (1) turns r over "original_max_position" rows L,
-                rotary_dim ln(L / (2 pi r)) / (2 ln theta), rounded down and up: what a
-                config.json means; and the rotated columns times "attention_factor"
+                rotary_dim ln(L / (2 pi r)) / (2 ln theta), rounded down and up (not with
+                "truncate" false): what a config.json means; and the rotated columns times "attention_factor"
                 (default 0.1 ln s + 1).  "ramp": "turns" instead of "pairs": a line in
                 the turns, g = (beta_fast - r) / (beta_fast - beta_slow)
     frequencies: a sequence of rotary_dim / 2 numbers instead of all that."""
@@ -87,20 +87,35 @@ class Rope:
     @classmethod
     def from_config(cls, config, layout: str = "half") -> "Rope":
         """From a model's config.json dict: rope_theta, partial_rotary_factor,
-        rope_scaling ({"rope_type" or "type": ..., "factor": ...,
-        "original_max_position_embeddings": ...})."""
+        rope_scaling ({"rope_type" or "type": ..., "factor": ..., ...}; yarn's first context is
+        "original_max_position_embeddings" rows, or the config's max_position_embeddings)."""
         dim = int(round(float(_cfg_get(config, "partial_rotary_factor", 0.25)) *
                         int(_cfg_get(config, "head_dim", HEAD_DIM))))
-        s = _cfg_get(config, "rope_scaling", None)
-        if s:
-            s = dict(s)
-            kind = s.pop("rope_type", None) or s.get("type", "default")
+        s = {k: v for k, v in (_cfg_get(config, "rope_scaling", None) or {}).items() if v is not None}
+        kind = s.pop("rope_type", None) or s.get("type", "default")
+        if kind == "default":
+            s = None
+        else:
             s["type"] = kind
-            if "original_max_position_embeddings" in s:
-                s["original_max_position"] = s.pop("original_max_position_embeddings")
-            if kind == "default":
-                s = None
+            rows = s.pop("original_max_position_embeddings", None)
+            if kind == "yarn":
+                _yarn_keys(s, rows or _cfg_get(config, "max_position_embeddings", None))
         return cls(dim, float(_cfg_get(config, "rope_theta", 1e7)), layout, s)
+
+
+def _yarn_keys(s: dict, rows) -> None:
+    """A config's keys of yarn as Rope's.  mscale and mscale_all_dim: the factor is
+    their ratio as 0.1 k ln s + 1 each; one of them alone (but for an mscale of 1) is read in
+    two ways, so it is refused."""
+    if rows is not None:
+        s["original_max_position"] = rows
+    a, b = s.pop("mscale", None), s.pop("mscale_all_dim", None)
+    if "attention_factor" in s or not (a or b) or (a == 1 and not b):
+        return
+    if not (a and b):
+        raise ValueError(f"yarn: mscale {a} with mscale_all_dim {b}: give attention_factor")
+    log = 0.1 * math.log(float(s.get("factor", 1.0)))
+    s["attention_factor"] = (a * log + 1.0) / (b * log + 1.0)
 
 
 def _scaled(dim: int, theta: float, scaling: dict):
@@ -111,7 +126,7 @@ def _scaled(dim: int, theta: float, scaling: dict):
             raise ValueError(f"scaling has no type but {sorted(scaling)}")
         return [theta ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0
     known = {"linear": set(), "ntk": set(),
-             "yarn": {"original_max_position", "beta_fast", "beta_slow", "ramp", "attention_factor"}}
+             "yarn": {"original_max_position", "beta_fast", "beta_slow", "ramp", "truncate", "attention_factor"}}
     if kind not in known:
         raise ValueError(f"scaling type {kind!r}: one of {sorted(known)}")
     if "factor" not in scaling:
@@ -139,7 +154,9 @@ def _scaled(dim: int, theta: float, scaling: dict):
         share = [(fast - rows * x / (2 * math.pi)) / (fast - slow) for x in f]
     elif ramp == "pairs":
         pair = [dim * math.log(rows / (2 * math.pi * r)) / (2 * math.log(theta)) for r in (fast, slow)]
-        first, last = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), dim - 1)
+        if scaling.get("truncate", True):
+            pair = [math.floor(pair[0]), math.ceil(pair[1])]
+        first, last = max(pair[0], 0), min(pair[1], dim - 1)
         if first > last and dim:
             raise ValueError(f"yarn: no pair of {dim} columns makes {slow} to {fast} turns in {rows} rows")
         share = [(i - first) / max(last - first, 0.001) for i in range(dim // 2)]

@@ -46,3 +46,40 @@ def test_yarn_by_turns_has_a_name_of_its_own():
             m.Rope(64, 1e6, scaling={"type": "yarn", "factor": 4.0, "original_max_position": 32768, **bad})
     with pytest.raises(ValueError):
         m.Rope(64, 1.0, scaling={"type": "yarn", "factor": 4.0, "original_max_position": 32768})
+
+
+def test_configs_as_models_have_them():
+    """Keys that such configs hold beside those that a type needs."""
+    for kind in ("linear", "ntk"):
+        r = m.Rope.from_config(config(rope_type=kind, factor=4.0, original_max_position_embeddings=32768))
+        assert r.frequencies == m.Rope(64, 1e7, scaling={"type": kind, "factor": 4.0}).frequencies
+    # no length of the first context: the config's own (262144)
+    r = m.Rope.from_config(config(type="yarn", factor=4.0, beta_fast=32, beta_slow=None))
+    assert math.isclose(r.frequencies[18], 1e7 ** (-18 / 32) * 0.625, rel_tol=1e-14)  # half way from 14 to 22
+    with pytest.raises(ValueError):
+        m.Rope.from_config({"rope_scaling": {"rope_type": "yarn", "factor": 4.0}})
+    # ends that are not rounded: 10.1125 and 16.9932 for 32768 rows
+    r = m.Rope.from_config(config(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768, truncate=False))
+    assert math.isclose(r.frequencies[14], 1e7 ** (-14 / 32) * (1 - 0.75 * (14 - 10.112548975) / 6.880685616), rel_tol=1e-9)
+    assert r.frequencies[11] < 1e7 ** (-11 / 32) and r.frequencies[16] > 0.25 * 1e7 ** (-16 / 32)
+
+
+@pytest.mark.parametrize("keys,factor", [
+    ({}, 1.1386294361119891), ({"attention_factor": 1.5}, 1.5), ({"attention_factor": None}, 1.1386294361119891),
+    ({"mscale": 1.0, "mscale_all_dim": 1.0}, 1.0), ({"mscale": 0.707, "mscale_all_dim": 0.707}, 1.0),
+    ({"mscale": 1.0, "mscale_all_dim": 0.5}, 1.1386294361119891 / 1.0693147180559945),  # 0.1 k ln 4 + 1 each
+    ({"mscale": 1.0}, 1.1386294361119891), ({"mscale": 1.0, "mscale_all_dim": 0}, 1.1386294361119891),
+    ({"mscale": 0.5, "mscale_all_dim": 1.0, "attention_factor": 2.0}, 2.0)])
+def test_yarn_factors(keys, factor):
+    r = m.Rope.from_config(config(rope_type="yarn", factor=4.0, original_max_position_embeddings=32768, **keys))
+    assert math.isclose(r.factor, factor, rel_tol=1e-15)
+
+
+@pytest.mark.parametrize("keys", [{"rope_type": "longrope", "factor": 4.0}, {"rope_type": "yarn"},
+                                  {"rope_type": "yarn", "factor": 4.0, "mscale": 0.5},  # read in two ways
+                                  {"rope_type": "yarn", "factor": 4.0, "mscale_all_dim": 0.5},
+                                  {"rope_type": "yarn", "factor": 4.0, "short_factor": [1.0]},
+                                  {"rope_type": "linear", "factor": 4.0, "beta_fast": 3}])
+def test_configs_that_are_refused(keys):
+    with pytest.raises(ValueError):
+        m.Rope.from_config(config(**keys))
