@@ -88,10 +88,15 @@ class Rope:
     def from_config(cls, config, layout: str = "half") -> "Rope":
         """From a model's config.json dict: rope_theta, partial_rotary_factor,
         rope_scaling ({"rope_type" or "type": ..., "factor": ..., ...}; yarn's first context is
-        "original_max_position_embeddings" rows, or the config's max_position_embeddings)."""
-        dim = int(round(float(_cfg_get(config, "partial_rotary_factor", 0.25)) *
-                        int(_cfg_get(config, "head_dim", HEAD_DIM))))
-        s = {k: v for k, v in (_cfg_get(config, "rope_scaling", None) or {}).items() if v is not None}
+        "original_max_position_embeddings" rows, or the config's max_position_embeddings), or
+        rope_parameters, which holds all three."""
+        s = _cfg_get(config, "rope_scaling", None) or _cfg_get(config, "rope_parameters", None) or {}
+        s = {k: v for k, v in s.items() if v is not None}
+        if any(isinstance(v, dict) for v in s.values()):
+            raise ValueError(f"rope_parameters of {sorted(s)}: give one layer type's")
+        theta = _cfg_get(config, "rope_theta", s.pop("rope_theta", 1e7))
+        part = _cfg_get(config, "partial_rotary_factor", s.pop("partial_rotary_factor", 0.25))
+        dim = int(round(float(part) * int(_cfg_get(config, "head_dim", HEAD_DIM))))
         kind = s.pop("rope_type", None) or s.get("type", "default")
         if kind == "default":
             s = None
@@ -100,7 +105,7 @@ class Rope:
             rows = s.pop("original_max_position_embeddings", None)
             if kind == "yarn":
                 _yarn_keys(s, rows or _cfg_get(config, "max_position_embeddings", None))
-        return cls(dim, float(_cfg_get(config, "rope_theta", 1e7)), layout, s)
+        return cls(dim, float(theta), layout, s)
 
 
 def _yarn_keys(s: dict, rows) -> None:

@@ -83,3 +83,17 @@ def test_yarn_factors(keys, factor):
 def test_configs_that_are_refused(keys):
     with pytest.raises(ValueError):
         m.Rope.from_config(config(**keys))
+
+
+def test_newer_configs_hold_all_of_it_in_one_place():
+    """rope_parameters: theta, the rotated part and the scaling."""
+    p = {"rope_type": "yarn", "rope_theta": 1e6, "partial_rotary_factor": 0.5, "factor": 4.0,
+         "original_max_position_embeddings": 32768}
+    for c in ({"head_dim": 256, "rope_parameters": p}, {"text_config": {"head_dim": 256, "rope_parameters": p}}):
+        r = m.Rope.from_config(c)
+        want = m.Rope(128, 1e6, scaling={"type": "yarn", "factor": 4.0, "original_max_position": 32768})
+        assert r.rotary_dim == 128 and r.frequencies == want.frequencies and r.factor == want.factor
+    r = m.Rope.from_config({"rope_parameters": {"rope_type": "default", "rope_theta": 1e4}})
+    assert r.frequencies == m.Rope(64, 1e4).frequencies
+    with pytest.raises(ValueError):  # one for each kind of layer
+        m.Rope.from_config({"rope_parameters": {"full_attention": p, "sliding_attention": p}})
