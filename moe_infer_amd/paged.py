@@ -80,9 +80,20 @@ class Rope:
         self.factor = float(turned if factor is None else factor)
         if not math.isfinite(self.factor):
             raise ValueError(f"factor {self.factor}")
-        self._f = (C.c_double * max(1, len(f)))(*f)
-        # the C arguments: frequencies, rotary_dim, interleaved, factor
-        self._args = (C.addressof(self._f), rotary_dim, int(layout == "interleaved"), self.factor)
+        self._pack()
+
+    def _pack(self) -> None:
+        """The C arguments: frequencies, rotary_dim, interleaved, factor."""
+        self._f = (C.c_double * max(1, len(self.frequencies)))(*self.frequencies)
+        self._args = (C.addressof(self._f), self.rotary_dim, int(self.layout == "interleaved"), self.factor)
+
+    # A copy makes its own: the address in _args is of this object's _f.
+    def __getstate__(self):
+        return {k: v for k, v in self.__dict__.items() if k not in ("_f", "_args")}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self._pack()
 
     @classmethod
     def from_config(cls, config, layout: str = "half") -> "Rope":

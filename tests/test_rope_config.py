@@ -1,6 +1,9 @@
 """Rotation plans from a model's config.json, against numbers written out from the
 formulas (no GPU)."""
+import copy
+import ctypes
 import math
+import pickle
 
 import pytest
 
@@ -97,3 +100,13 @@ def test_newer_configs_hold_all_of_it_in_one_place():
     assert r.frequencies == m.Rope(64, 1e4).frequencies
     with pytest.raises(ValueError):  # one for each kind of layer
         m.Rope.from_config({"rope_parameters": {"full_attention": p, "sliding_attention": p}})
+
+
+def test_a_copied_plan_has_frequencies_of_its_own():
+    """What the C entry reads lives as long as the copy, whatever becomes of the original."""
+    r = m.Rope(64, 1e6, "interleaved", {"type": "linear", "factor": 2.0})
+    for other in (copy.deepcopy(r), copy.copy(r), pickle.loads(pickle.dumps(r))):
+        assert other.frequencies == r.frequencies and other.layout == r.layout and other.factor == r.factor
+        at, rotary_dim, interleaved, factor = other._args
+        assert at == ctypes.addressof(other._f) != ctypes.addressof(r._f)
+        assert tuple(other._f) == r.frequencies and (rotary_dim, interleaved, factor) == (64, 1, 1.0)
