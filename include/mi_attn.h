@@ -384,9 +384,11 @@ mi_status mi_rope_apply(const void* x, int32_t x_type, int64_t token_stride, int
 
 /* Appends n tokens' K and V: K RMS-normed (k_norm_w, bf16 [D] or NULL), rotated
  * at its row (as mi_rope_apply) and quantised, V quantised.  Scale and offset of
- * a group: f16((max - min) / 15), f16(min - 16 scale); code: the nearest, ties to
- * even; 64-bit arithmetic throughout.  A group that holds a NaN or an infinity,
- * or whose scale or offset does not fit f16, is stored as NaN.  With q: q_out
+ * a group: f16((max - min) / 15), f16(min - 16 scale), which is lowered to the
+ * largest f16 not above 65504 - 31 scale where code 15 would stand for a value past
+ * f16; code: the nearest, ties to even; 64-bit arithmetic throughout.  A group that
+ * holds a NaN or a value that rounds past f16, or whose scale or offset does not
+ * fit it, is stored as NaN.  With q: q_out
  * [n][H][D] f16 = q normed (q_norm_w) and rotated, in the same launch; q_out may
  * be q (contiguous f16).  q, k, v: one mi_dtype, strides as for mi_rope_apply.
  * Rows outside the call's keep their contents.  Beside kv_cache_append

@@ -62,10 +62,13 @@ struct AppendArgs {
   mi::RotaryPlan plan;
 };
 
-// x rounded once to f16 (the conversion goes by way of f32 and rounds twice).
+// x rounded once to f16, to the nearest or down (the conversion goes by way of f32 and
+// rounds twice).
+template <bool DOWN = false>
 __device__ __forceinline__ _Float16 f64_to_f16(double x) {
   const int bits = 11 - max(__builtin_amdgcn_frexp_exp(x), -13);
-  return (_Float16)(float)ldexp(rint(ldexp(x, bits)), -bits);
+  const double y = ldexp(x, bits);
+  return (_Float16)(float)ldexp(DOWN ? floor(y) : rint(y), -bits);
 }
 
 struct Quant {
@@ -80,7 +83,14 @@ __device__ __forceinline__ Quant quantise(const double (&z)[4], double lo, doubl
   // reciprocal lacks
   const double range = hi - lo, q = range * (1.0 / 15.0);
   const double scale = (double)f64_to_f16(fma(fma(-15.0, q, range), 1.0 / 15.0, q));
-  const double offset = (double)f64_to_f16(lo - 16.0 * scale);
+  double offset = (double)f64_to_f16(lo - 16.0 * scale);
+  // Code 15 stands for a value of f16: next to the end of its range the roundings of scale
+  // and offset, which move it by less than 50, would put it past, an infinity from values
+  // that are none.
+  if (__any(hi > 64000.0)) {
+    if (fma(31.0, scale, offset) >= 65520.0) offset = (double)f64_to_f16<true>(fma(-31.0, scale, 65504.0));
+    fine = fine && hi < 65520.0;
+  }
   const uint64_t ok = __ballot(fine) >> (threadIdx.x & 48);
   if ((ok & 0xffff) != 0xffff || !(fabs(offset) < __builtin_inf()) || !(scale < __builtin_inf())) {
     const _Float16 bad = (_Float16)__builtin_nanf("");
