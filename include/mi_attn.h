@@ -365,6 +365,9 @@ mi_status mi_rope_apply(const void* x, int32_t x_type, int64_t token_stride, int
  *     4-bit codes of K (4096 bytes) and V (4096), then scales and offsets in f16
  *     per row and group of 64 columns, of K (512) and V (512).  A value is
  *     f16((16 + code) * scale + offset).  csrc/paged.h has the order within a tile.
+ *     31 * scale + offset is within f16 in what mi_paged_append writes; where a caller
+ *     fills in others, tokens that see the row read NaN or infinities of that group
+ *     beside its values, and those that do not see it are untouched.
  *   block_table: int32 [batch][table_cols], the page of rows
  *     [j page_rows, (j + 1) page_rows) of a sequence; unused entries -1.
  *   kv_len: int32 [batch], rows of each sequence, those of this call included.

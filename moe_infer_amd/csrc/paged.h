@@ -97,6 +97,13 @@ __device__ __forceinline__ f16x2 pk_fma(f16x2 a, f16x2 b, f16x2 c) {
   return __builtin_elementwise_fma(a, b, c);
 }
 
+// The top bits of the halves (rows) of scales s and offsets o whose code 15, the one
+// furthest out, stands for no finite value (an exponent that is all ones carries there).
+__device__ __forceinline__ uint32_t past_f16(uint32_t s, uint32_t o) {
+  const f16x2 top = pk_fma(f16x2{31, 31}, __builtin_bit_cast(f16x2, s), __builtin_bit_cast(f16x2, o));
+  return ((__builtin_bit_cast(uint32_t, top) & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+}
+
 // Eight values of one scale and offset, in the order {0,4,1,5,2,6,3,7} of the
 // word's nibbles.
 __device__ __forceinline__ f16x8 dequant_row(uint32_t w, f16x2 scale, f16x2 offset,

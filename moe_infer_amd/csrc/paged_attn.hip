@@ -200,28 +200,28 @@ struct Wave {
     for (int g = 0; g < 4; g++) {
       f16x8 vs = b.vs[g], vo = b.vo[g];
       bool odd_group = false;
-      uint32_t poison = 0;  // columns that see a value of this group that is not finite
+      uint32_t poison = 0;  // columns that see a row whose values of this group may not be finite
       if constexpr (MASKED) {
-        // V is cleared where no column sees the row or where it is not finite (its MFMA
+        // V is cleared where no column sees the row or where it may not be finite (its MFMA
         // would make NaN of 0 * NaN); columns that do see such a row get their NaN
-        // here.  In pairs of rows (4 quad + i, 16 more), as the scales lie; a half
-        // whose exponent is all ones carries into its top bit.
+        // here.  What tells is the value of code 15, the furthest of the sixteen from
+        // 0 once one of them is past f16.  In pairs of rows (4 quad + i, 16 more), as the
+        // scales lie; a half whose exponent is all ones carries into its top bit.
         u32x4 ws = __builtin_bit_cast(u32x4, vs), wo = __builtin_bit_cast(u32x4, vo);
-        uint32_t odd = 0;
+        uint32_t top[4], odd = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           ws[i] &= in1[i];
           wo[i] &= in1[i];
-          odd |= ((ws[i] & 0x7c007c00u) + 0x04000400u) | ((wo[i] & 0x7c007c00u) + 0x04000400u);
+          const uint32_t s = ws[i], o = wo[i];
+          top[i] = mi::past_f16(s, o);
+          odd |= top[i];
         }
-        odd_group = __any((odd & 0x80008000u) != 0);
+        odd_group = __any(odd != 0);
         if (odd_group) {
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const uint32_t top = (((ws[i] & 0x7c007c00u) + 0x04000400u) |
-                                  ((wo[i] & 0x7c007c00u) + 0x04000400u)) &
-                                 0x80008000u;
-            const uint32_t halves = (top >> 15) * 0xffffu;
+            const uint32_t halves = (top[i] >> 15) * 0xffffu;
 #pragma unroll
             for (int ct = 0; ct < CT; ct++)
               if (halves & seen(row0 + 4 * quad + i, lim[ct])) poison |= 1u << ct;

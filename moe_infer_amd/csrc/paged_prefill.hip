@@ -104,7 +104,7 @@ __device__ __forceinline__ void mfma_s0(f32x16& c, f16x8 a, f16x8 b) {
 template <int KP>
 __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a, const PrefillExtra x) {
   extern __shared__ char lds[];  // K, V [2][2 halves], their scales; then the join of the key halves
-  __shared__ int odd_row[4];  // least masked row whose V group is not finite
+  __shared__ int odd_row[4];  // least masked row whose V group may not be finite
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int kRows = rows_of(KP), kKeys = 32 * KP;
   const int qb = KP == 1 ? w : w & 1, kp = KP == 1 ? 0 : w >> 1;
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
     char* const vsc = ksc + 1024 * KP;
     auto put_sk = [&](int t, uint32_t y) { *(uint32_t*)(ksc + (t & 1) * 512 * KP + (KP == 2 ? 4 * tid : sat)) = y; };
     // V's word: scale or offset of rows 4 quad + i and 16 more, of group g.  Rows that no
-    // token of the block sees read as zero, and so does what is not finite in rows that
+    // token of the block sees read as zero, and so do values that may not be finite in rows that
     // some token does not see (the MFMA would make NaN of 0 * NaN for it); the
     // tokens that do see such a row get their NaN at the end.
     auto put_sv = [&](int t, uint32_t y) {
@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         const int i = x & 3, sq = (x >> 3) & 3, g = (x >> 5) & 3;
         const int row = kKeys * t + (KP == 2 ? 32 * su : 0) + 4 * sq + i;
         y &= (row < end ? 0xffffu : 0u) | (row + 16 < end ? 0xffff0000u : 0u);
-        const uint32_t odd = ((y & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+        const bool is_offset = x & 4;  // the scale's or the offset's other word is four lanes away
+        const uint32_t other = __shfl_xor((int)y, 4, 64);
+        const uint32_t odd = mi::past_f16(is_offset ? other : y, is_offset ? y : other);
         if (odd) {
           atomicMin(&odd_row[g], odd & 0x8000u ? row : row + 16);
           y &= ~((odd >> 15) * 0xffffu);

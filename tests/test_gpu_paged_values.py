@@ -5,8 +5,9 @@ import torch
 
 import moe_infer_amd as m
 
+from . import paged_ref as R
 from .gpu_util import announce
-from .test_gpu_paged import D, Pool, f64, i32
+from .test_gpu_paged import D, Pool, f64, gen, i32, near, poison_tail, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,41 @@ def test_finite_values_read_back_finite(dtype, ragged):
         fine = ~np.isnan(want).any(1)
         assert np.all(np.isfinite(got[fine])) and (name == "v" or fine.mean() > 0.95)
         assert np.all(np.abs(got - src)[fine] <= (np.maximum(0.5 * s, 64) + 16)[fine]), name
+
+
+# -------------------------------------------------------------- attention --
+
+def large_group(pool, s, row, head, group, col):
+    """V of a row's group: 16 scales of 1000 past 40000, but for column `col`, 31 of them."""
+    page, t, w = pool.table[s][row // pool.page_rows], row % pool.page_rows // 32, row % 32
+    tile = pool.host[page, head, t]
+    h, words = tile.view(np.float16), tile.view(np.uint32)
+    so = R.V_SO[w][64 * group]
+    h[so], h[so + 8] = 1000.0, 40000.0
+    for c in range(64 * group, 64 * group + 64):
+        word, nib = R.V_WORD[w][c], int(R.V_NIB[w][c])
+        words[word] = np.uint32((int(words[word]) & ~(15 << (4 * nib))) | ((15 << (4 * nib)) if c == col else 0))
+
+
+@pytest.mark.parametrize("new,past", [(2, 62), (3, 62), (16, 56), (60, 40), (100, 40), (100, 3000)])
+def test_large_values_do_not_reach_those_before_them(new, past):
+    """A value past f16's range in a row that the later tokens see and the earlier do not: its
+    scale and offset are finite, its product with a weight of 0 is not."""
+    announce(f"{new} tokens behind {past}")
+    lens = [new + past, 70]
+    pool = Pool(3, lens, page_rows=32)
+    poison_tail(pool, lens)
+    q = randn(gen(4), new + 2, 16, D)
+    ref, limit = pool.reference(q, [new, 2])
+    row, group, col = past + new - 1 if new < 16 else past + new // 2, 2, 2 * 64 + 5
+    seen = row - past
+    large_group(pool, 0, row, 1, group, col)
+    pool.put()
+    for bound in (max(lens), 1 << 24):
+        out = f64(m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of([new, 2]), q, new, bound))
+        near(out[:seen], ref[:seen], limit[:seen], "tokens before it")
+        near(out[:, :8], ref[:, :8], limit[:, :8], "the other KV head")
+        near(out[new:], ref[new:], limit[new:], "the other sequence")
+        rest = np.r_[0:128, 192:256]
+        near(out[seen:new, 8:][..., rest], ref[seen:new, 8:][..., rest], limit[seen:new, 8:][..., rest], "other groups")
+        assert not np.any(np.isfinite(out[seen:new, 8:, col])), "tokens that see it"
