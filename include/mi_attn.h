@@ -417,7 +417,8 @@ mi_status mi_paged_read(const void* pages, int64_t num_pages, int32_t page_rows,
 
 /* Attention of the call's tokens over the pages: token i of sequence s attends
  * the rows up to its own, softmax(q . K^T / sqrt(D)) V, then out *= sigmoid(gate)
- * when gate != NULL (f16 or f32: gate_type).  cu_q == NULL is a decode step (one
+ * when gate != NULL (f16 or f32: gate_type); a token that attends nothing gives
+ * zeros, whatever its gate holds.  cu_q == NULL is a decode step (one
  * token per sequence); prompts, chunks behind cached rows and drafts to verify go
  * through cu_q.  max_q, max_len: at least every sequence's tokens and rows (a
  * sequence beyond them gets NaN).  q: f16 [n][H][D], q and gate strided as for

@@ -28,9 +28,11 @@ __device__ __forceinline__ f32x4 gate4(const AttnArgs& a, int64_t gi) {
   return f32x4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
 }
 
-// out of four columns: the gate, then f16.
-__device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x) {
-  if (a.gate) {
+// out of four columns: their sums x times inv, the weights' sum's inverse, the gate, then
+// f16.  inv is 0 for a token that attends nothing: zeros, whatever its gate holds.
+__device__ __forceinline__ void put4(const AttnArgs& a, int64_t tok, int head, int d, f32x4 x, float inv) {
+  x *= inv;
+  if (a.gate && inv != 0.f) {
     const f32x4 g = gate4(a, tok * a.g_ts + head * a.g_hs + d);
 #pragma unroll
     for (int e = 0; e < 4; e++) x[e] = gate_mul(x[e], g[e]);

@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
         if (whole) {
           const int tok = col / a.R;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, x * inv);
+          mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, x, inv);
         } else {
           *(f32x4*)(a.part_o + (col0 + 16 * ct + c) * D + d) = x;
           if (d == 0) *(float2*)(a.part_ml + (col0 + 16 * ct + c) * 2) = float2{tbox[c], sum};
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
     y += acc[g * d4 + t] * f;
   }
   const int tok = col / a.R;
-  mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y * (total == 0.f ? 0.f : 1.f / total));
+  mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y, total == 0.f ? 0.f : 1.f / total);
 }
 
 // Columns that the decode kernels take at most (two blocks of 16).

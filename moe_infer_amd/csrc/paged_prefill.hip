@@ -539,7 +539,8 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
         }
       mi::sync_lds();
     }
-    const bool early = whole && a.gate && !a.gate32;
+    // (Tokens without a row, whose gates may hold anything, are zero whatever those are.)
+    const bool early = whole && a.gate && !a.gate32 && first >= 0;
     int r0 = 64 * qb + 32 * kp;
     // Lane i's: where row r0 + i (or the last one) lies in the gate and in the output.
     int64_t gate_at, out_at;
@@ -665,8 +666,8 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(const AttnArgs a,
 #pragma unroll 1
           for (int i = 0; i < 32; i++) {
             f32x4 y = mine[64 * i + (lane ^ (i & 7))];
-            if (a.gate) {
-              const f32x4 g = *(const f32x4*)((const float*)a.gate + lane64(gate_at, i) + 4 * lane);
+            if (a.gate && first + mi::uniform(token(r0 + i)) >= 0) {
+              const f32x4 g = mi::gate4(a, lane64(gate_at, i) + 4 * lane);
 #pragma unroll
               for (int e = 0; e < 4; e++) y[e] = mi::gate_mul(y[e], g[e]);
             }
@@ -763,7 +764,7 @@ __global__ void __launch_bounds__(256) paged_prefill_merge_kernel(const AttnArgs
     const float f = __builtin_amdgcn_exp2f(t - mn), g = __builtin_amdgcn_exp2f(ml.x - mn);
     const float all = l * f + ml.y * g, inv = all == 0.f ? 0.f : 1.f / all;
     f32x4 z = ((half ? y[2 + i] : y[i]) * f + box[w & 1][j][lane] * g) * inv;
-    if (a.gate)
+    if (a.gate && inv != 0.f)  // zeros where a token attends nothing
 #pragma unroll
       for (int e = 0; e < 4; e++) z[e] = mi::gate_mul(z[e], gate[i][e]);
     *(f16x4*)(a.out + out_at[i]) = f16x4{(_Float16)z[0], (_Float16)z[1], (_Float16)z[2], (_Float16)z[3]};

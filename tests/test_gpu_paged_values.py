@@ -108,3 +108,24 @@ def test_large_values_do_not_reach_those_before_them(new, past):
         rest = np.r_[0:128, 192:256]
         near(out[seen:new, 8:][..., rest], ref[seen:new, 8:][..., rest], limit[seen:new, 8:][..., rest], "other groups")
         assert not np.any(np.isfinite(out[seen:new, 8:, col])), "tokens that see it"
+
+
+@pytest.mark.parametrize("bound", [100, 6000])  # an item to a workgroup, and split
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_without_keys_are_zero_whatever_their_gate(bound, dtype):
+    """A padded batch: empty sequences and tokens without a row, whose gates nobody wrote."""
+    lens, new = [0, 70, 3, 64], [2, 2, 5, 200]
+    pool = Pool(5, [0, 70, 3, 64])
+    g = gen(6)
+    for count in (1, 2, 5, 200):
+        take = [min(a, count) for a in new]
+        n = sum(take)
+        q, gate = randn(g, n, 16, D), randn(g, n, 16, D, dtype=dtype)
+        first = np.concatenate([[r - a + i for i in range(a)] for r, a in zip(lens, take)])
+        none = torch.from_numpy(first < 0).cuda()
+        gate[none] = float("nan")
+        out = f64(m.attn_prefill_paged(pool.pages, pool.t, pool.len, cu_of(take), q, count, bound, gate=gate))
+        gate[none] = 0.0
+        ref, limit = pool.reference(q, take, gate)
+        near(out, ref, limit, f"at most {count} tokens")
+        assert np.all(out[first < 0] == 0)
