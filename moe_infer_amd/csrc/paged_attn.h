@@ -17,8 +17,8 @@ struct AttnArgs {
   _Float16* out;     // [n][G R][D]
   float* part_o;     // [2 workgroups][16 CT][D]
   float* part_ml;    // [2 workgroups][16 CT][2]
-  int2* seg;         // [batch G ncb]: first slot and last workgroup of an item, or -1
-  int32_t n, R, max_q, max_len, wgs, ncb, gate32, dsplit;
+  int2* seg;         // [batch G]: first slot and last workgroup of an item, or -1
+  int32_t n, R, max_q, max_len, wgs, gate32, dsplit;
 };
 
 // Four values of the gate, from element gi on.

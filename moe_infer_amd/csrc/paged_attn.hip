@@ -1,9 +1,9 @@
-// Attention over the paged 4-bit cache (paged.h): decode steps, drafts to
-// verify, chunks and prompts.
+// Attention over the paged 4-bit cache (paged.h): decode steps and drafts to verify, up
+// to 32 columns a sequence and KV head.
 //
-// The columns of a (sequence, KV head) are its (token, query head of the
-// group) pairs, token-major; a workgroup takes CT blocks of 16 of them and a
-// range of 32-row tiles, which its waves take in turn.  A wave's tile:
+// The columns are its (token, query head of the group) pairs, token-major; a workgroup
+// takes all of them, in CT blocks of 16, and a range of 32-row tiles, which its waves
+// take in turn.  A wave's tile:
 //   S [32 keys x 16 CT] = K Q^T    16x16x32 MFMA, K dequantised in registers
 //   running maximum and sum per column (f32), P = 2^(S - max) in f16
 //   O^T [256 x 16 CT] += V^T P     V dequantised in registers
@@ -44,14 +44,12 @@ constexpr int ahead(int ct) { return ct == 1 ? 1 : 2; }
 // Tiles below which a workgroup is not split further: one to a wave.
 constexpr int kMinTiles = 8;
 
-// A sequence as its work: ncb blocks of 16 CT columns per KV head, each over
-// ntiles tiles of 32 rows.  Items of a sequence are (KV head, block); its weight,
-// items times tiles over the KV heads, is ncb * ntiles.
+// A sequence as its work: ntiles tiles of 32 rows for each KV head, its items.
 struct Seq {
-  int q0, nq, len, ncb, ntiles;
+  int q0, nq, len, ntiles;
   bool bad;  // beyond max_q or max_len
 };
-template <int CT, bool UNIFORM>
+template <bool UNIFORM>
 __device__ __forceinline__ Seq get_seq(const AttnArgs& a, int s) {
   auto load = [](const int32_t* p) { return UNIFORM ? mi::uniform_load(p) : *p; };
   Seq r;
@@ -60,8 +58,7 @@ __device__ __forceinline__ Seq get_seq(const AttnArgs& a, int s) {
   r.len = load(a.pv.kv_len + s);
   r.bad = r.len < 0 || r.len > a.max_len || r.nq > a.max_q;
   if (r.nq <= 0 || r.q0 < 0 || (int64_t)r.q0 + r.nq > a.n) r.nq = 0;
-  r.ncb = r.bad ? 0 : (r.nq * a.R + 16 * CT - 1) / (16 * CT);
-  r.ntiles = r.bad ? 0 : (r.len + 31) >> 5;
+  r.ntiles = r.bad || r.nq == 0 ? 0 : (r.len + 31) >> 5;
   return r;
 }
 
@@ -280,7 +277,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
 
   // By chunks: every item in chunks of up to kMinTiles tiles, one to a workgroup,
   // where the grid has that many.  Else a flat line of tiles, [sequence][KV
-  // head][block][tile], in even pieces, one to a workgroup.
+  // head][tile], in even pieces, one to a workgroup.
   int s = 0, before = 0, f = 0, f1 = 0;
   const int G = a.pv.G;
   bool chunks = true;
@@ -291,10 +288,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
   } else {
     mi::find_seq<NT>(
         a.pv.batch,
-        [&](int i) {
-          const Seq q = get_seq<CT, false>(a, i);
-          return q.ncb * parts(q.ntiles);
-        },
+        [&](int i) { return parts(get_seq<false>(a, i).ntiles); },
         [&](int total) {
           chunks = (uint32_t)total * G <= (uint32_t)a.wgs;
           f = bid;
@@ -305,10 +299,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
     if (!chunks)
       mi::find_seq<NT>(
           a.pv.batch,
-          [&](int i) {
-            const Seq q = get_seq<CT, false>(a, i);
-            return q.ncb * q.ntiles;
-          },
+          [&](int i) { return get_seq<false>(a, i).ntiles; },
           [&](int total) {
             const uint32_t all = (uint32_t)total * G, each = all / a.wgs, more = all - each * a.wgs;
             f = (int)(each * bid + min((uint32_t)bid, more));
@@ -323,36 +314,33 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
   Wave<CT> st;
   st.x16 = mi::sixteens();
   while (f < f1) {
-    int h, cb, t0, t1;
+    int h, t0, t1;
     Seq sq;
     if constexpr (SINGLE) {
-      s = (int)((uint32_t)f / (uint32_t)(G * a.ncb));
-      const int vh = f - s * G * a.ncb;
-      h = (int)((uint32_t)vh / (uint32_t)a.ncb);
-      cb = vh - h * a.ncb;
-      sq = get_seq<CT, true>(a, s);
+      s = (int)((uint32_t)f / (uint32_t)G);
+      h = f - s * G;
+      sq = get_seq<true>(a, s);
       t0 = 0;
       t1 = sq.ntiles;
       f = f1;
       if (sq.bad) {
         const int width = a.R * D;
-        for (int tok = 0; tok < (cb ? 0 : sq.nq); tok++)
+        for (int tok = 0; tok < sq.nq; tok++)
           for (int i = threadIdx.x; i < width; i += NT)
             a.out[((int64_t)(sq.q0 + tok) * G + h) * width + i] = (_Float16)__builtin_nanf("");
         return;
       }
-      if (cb >= sq.ncb) return;
+      if (sq.nq == 0) return;
     } else {
-      sq = get_seq<CT, true>(a, s);
-      const int per = chunks ? parts(sq.ntiles) : sq.ntiles, weight = sq.ncb * per;
-      if (f >= G * (before + weight)) {
-        before += weight;
+      sq = get_seq<true>(a, s);
+      const int per = chunks ? parts(sq.ntiles) : sq.ntiles;
+      if (f >= G * (before + per)) {
+        before += per;
         s++;
         continue;
       }
-      const uint32_t local = f - G * before, vh = local / (uint32_t)per, at = local - vh * per;
-      h = (int)(vh / (uint32_t)sq.ncb);
-      cb = (int)vh - h * sq.ncb;
+      const uint32_t local = f - G * before, head = local / (uint32_t)per, at = local - head * per;
+      h = (int)head;
       if (chunks) {
         t0 = (int)(at * (uint32_t)sq.ntiles / (uint32_t)per);
         t1 = (int)((at + 1) * (uint32_t)sq.ntiles / (uint32_t)per);
@@ -363,13 +351,13 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
         f += t1 - t0;
       }
     }
-    const int c0 = cb * 16 * CT, ncols = sq.nq * a.R, first = sq.len - sq.nq;
+    const int ncols = sq.nq * a.R, first = sq.len - sq.nq;
 
     // the lane's columns: their rows of Q, and the rows they see (columns past the
     // last take the first's, which nothing reads)
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
-      const int c = c0 + 16 * ct + (lane & 15);
+      const int c = 16 * ct + (lane & 15);
       const bool in = c < ncols;
       const int tok = in ? c / a.R : 0, head = h * a.R + (in ? c - tok * a.R : 0);
       st.lim[ct] = in ? first + tok + 1 : 0;
@@ -377,8 +365,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
 #pragma unroll
       for (int i = 0; i < 8; i++) st.q[ct][i] = *(const f16x8*)(qp + 64 * (i >> 1) + 8 * (i & 1));
     }
-    const int lim0 = first + c0 / a.R + 1;                                       // first column's
-    const int lim1 = first + min(sq.nq - 1, (c0 + 16 * CT - 1) / a.R) + 1;       // last column's
+    const int lim0 = first + 1, lim1 = sq.len;  // first and last token's
     // tiles [t0, tm) are seen whole, [tm, t1) not
     const int tm = max(t0, min(t1, lim0 >> 5));
 
@@ -468,7 +455,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       __syncthreads();
       const int d = 4 * (tid & 63);
       for (int c = w; c < mcols; c += NW) {
-        const int col = c0 + 16 * ct + c;
+        const int col = 16 * ct + c;
         if (col >= ncols) break;
         float sum = 0.f;
         f32x4 x = {};
@@ -489,7 +476,7 @@ __global__ void __launch_bounds__(64 * waves(CT), CT == 1 ? 2 : 1) paged_attn_ke
       __syncthreads();
     }
     if (!SINGLE && threadIdx.x == 0) {  // where the merge finds the item's pieces
-      int2* const sg = a.seg + ((int64_t)s * G + h) * a.ncb + cb;
+      int2* const sg = a.seg + (int64_t)s * G + h;
       if (whole) {
         sg->x = -1;
       } else {
@@ -512,15 +499,14 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
   const uint32_t parts = a.dsplit, d4 = 64 / parts, groups = 256 / d4;
   const uint32_t bid = blockIdx.y * gridDim.x + blockIdx.x;  // below 2^31 (make_plan)
   const uint32_t ic = bid / parts, part = bid - ic * parts;
-  const uint32_t item = ic / (16 * CT), c = ic % (16 * CT);
-  if (item >= (uint32_t)a.pv.batch * a.pv.G * a.ncb) return;
-  const uint32_t sh = item / a.ncb, cb = item - sh * a.ncb;
-  const int s = sh / a.pv.G, h = sh - s * a.pv.G;
-  const Seq sq = get_seq<CT, true>(a, s);
-  const int col = cb * 16 * CT + c;
+  const uint32_t item = ic / (16 * CT);
+  const int col = ic % (16 * CT);
+  if (item >= (uint32_t)a.pv.batch * a.pv.G) return;
+  const int s = item / a.pv.G, h = item - s * a.pv.G;
+  const Seq sq = get_seq<true>(a, s);
   const uint32_t t = threadIdx.x, lane4 = t % d4, grp = t / d4, d = 4 * (part * d4 + lane4);
-  if (sq.bad || sq.ntiles == 0) {  // every token of the sequence, by its items' first workgroups
-    if (cb || c || part) return;
+  if (sq.bad || sq.ntiles == 0) {  // every token of the sequence, by its items' first workgroup
+    if (col || part) return;
     const _Float16 x = sq.bad ? (_Float16)__builtin_nanf("") : (_Float16)0.f;
     const int width = a.R * D;
     for (int tok = 0; tok < sq.nq; tok++)
@@ -532,7 +518,7 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
   const int2 sg = a.seg[item];
   if (sg.x < 0) return;
   const int first = sg.x >> 1, count = sg.y - first + 1;
-  auto slot = [&](int i) { return (i ? 2 * (first + i) : sg.x) * (16 * CT) + (int)c; };
+  auto slot = [&](int i) { return (i ? 2 * (first + i) : sg.x) * (16 * CT) + col; };
   float top = kNegBig, sum = 0.f;
   f32x4 x = {};
   for (int i0 = grp; i0 < count; i0 += 4 * (int)groups) {
@@ -580,10 +566,12 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const AttnArgs a) {
   mi::put4(a, sq.q0 + tok, h * a.R + col - tok * a.R, d, y, total == 0.f ? 0.f : 1.f / total);
 }
 
-// Columns that the decode kernels take at most (two blocks of 16).
+// Columns of a sequence and KV head that the decode kernels take at most: a workgroup
+// takes them all.
 constexpr int kManyColumns = 32;
 
-// Column blocks of 16 a workgroup takes: 2 where a sequence has more than one.
+// Column blocks of 16 a workgroup takes.
+static_assert(kManyColumns == 2 * 16, "a workgroup of two blocks takes every column");
 int column_blocks(int32_t max_q, int R) { return (int64_t)max_q * R <= 16 ? 1 : 2; }
 
 // Whether the prompts' form serves a call: 16 sequences of 4 tokens, 8 heads a group,
@@ -591,7 +579,7 @@ int column_blocks(int32_t max_q, int R) { return (int64_t)max_q * R <= 16 ? 1 : 
 bool many_columns(int32_t max_q, int R) { return (int64_t)max_q * R > kManyColumns; }
 
 struct Plan {
-  int ct, ncb, wgs, dsplit;
+  int ct, wgs, dsplit;
   bool single;
   int64_t items, tiles;
   size_t o_bytes, ml_bytes, seg_bytes;
@@ -602,8 +590,7 @@ Plan make_plan(int32_t batch, int32_t max_q, int32_t max_len, int H, int G) {
   Plan p;
   const int R = H / G;
   p.ct = column_blocks(max_q, R);
-  p.ncb = (int)(((int64_t)max_q * R + 16 * p.ct - 1) / (16 * p.ct));
-  p.items = (int64_t)batch * G * p.ncb;
+  p.items = (int64_t)batch * G;
   p.tiles = p.items * (((int64_t)max_len + 31) / 32);
   const int64_t per_item = (((int64_t)max_len + 31) / 32 + kMinTiles - 1) / kMinTiles;
   p.wgs = (int)std::max<int64_t>(1, std::min<int64_t>(256, p.items * per_item));
@@ -725,7 +712,6 @@ extern "C" mi_status mi_attn_paged(
   a.max_len = max_len;
   a.seg = (int2*)((char*)workspace + p.o_bytes + p.ml_bytes);
   a.wgs = p.wgs;
-  a.ncb = p.ncb;
   a.dsplit = p.dsplit;
   const hipStream_t s = (hipStream_t)stream;
   if (many) return mi::paged_prefill(a, workspace, s);
