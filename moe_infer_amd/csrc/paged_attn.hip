@@ -16,13 +16,13 @@
 // partials that paged_merge_kernel joins.
 //
 // Bound: for one column block, the page bytes and what a wave issues for them (64
-// sequences of up to 32768 rows, 640 MB: 126.5 us, 5.1 TB/s; a wave's
+// sequences of up to 32768 rows, 640 MB: 126 us, 5.1 TB/s; a wave's
 // tile is 5300 clocks, two waves to a SIMD, of which 680 wait for memory and 13 % of the
 // walk goes to waiting at the join for the SIMD's other wave).  For two, one wave's
 // instructions (16 sequences of 4 tokens behind up to 32768 rows, 188 MB: 72 us and 5 of
 // merge; 4850 clocks a tile, 990 of them waiting).  For few tiles, the chain from the tables
-// to a page's id, its tile and the join: 8 sequences of up to 777 rows 10.3 us, one of
-// 32768 rows 12.3 and 4.9 of merge.
+// to a page's id, its tile and the join: 8 sequences of up to 512 rows 10.4 us, one of
+// 32768 rows 13.3 and 4.8 of merge (both as traced).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -75,8 +75,9 @@ struct Tile {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, p ? mi::kTileBytes : 0,
                                              0x00020000);
   }
-  // (Past the caches, bit 1: a call reads a page's bytes once.  64 sequences 126.5 us, 133.7
-  // without; the same for the small ones.)
+  // (Past the caches, bit 1: a call reads a sequence's page bytes once.  64 sequences 126.5
+  // us, 133.7 without; the same for the small ones.  A page that sequences share is read
+  // by each of them, which was not timed.)
   static __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t b, int lane_at, int at) {
     return __builtin_amdgcn_raw_buffer_load_b128(b, lane_at + at, 0, 2);
   }

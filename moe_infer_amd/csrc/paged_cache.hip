@@ -395,8 +395,8 @@ struct ReadArgs {
 // Rows of one tile of one sequence and KV head as f16: waves 0 and 1 take K, a
 // thread eight words of rows 16 apart in steps of 4; waves 2 and 3 take V, a thread eight
 // rows of eight columns.  Bound: memory (66,000 rows of two KV heads, 38 MB in and 135
-// out, 30.5 us; the rows are stored past the caches, which they would only sweep: 42.2
-// without).
+// out, 31 us; the rows are stored past the caches, which they would only sweep: 42.2
+// without, for the call alone; small calls take the same way).
 __global__ void __launch_bounds__(256) paged_read_kernel(const ReadArgs a) {
   const int t = threadIdx.x;
   const int64_t item = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;

@@ -192,7 +192,8 @@ __device__ __forceinline__ uint16_t f32_to_bf16(float x) {  // nearest, ties to 
   return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
 }
 // PAST: past the caches, for more rows than they keep (4099 tokens of 16 heads 18.6 us
-// without and 17.9; prompts of 6580 tokens appended 31.4 and 29.1).
+// without and 17.9; prompts of 6580 tokens appended 31.4 and 29.1: the calls alone, without
+// the one that reads the rows next).
 template <bool PAST, typename V>
 __device__ __forceinline__ void put(V* p, V x) {
   if constexpr (PAST) __builtin_nontemporal_store(x, p);

@@ -13,7 +13,8 @@ attn_decode_paged.  The tables live on the device and the kernels read them, so
 a captured step follows them as the program updates them in place.
 
 PagedCache owns the pages of all layers and deals them to sequences;
-PagedCache.batch() makes the tables of a step.  The functions take tensors, so
+PagedCache.batch() makes the tables of a step, new tensors each time: for a captured
+step, copy them into its own (the block table into the first of its columns).  The functions take tensors, so
 a program with an allocator of its own needs only the layout (include/mi_attn.h).
 
 Beside the single-sequence Cache / qk_norm_rope_append / attn_prefill and the
