@@ -53,9 +53,9 @@ class Rope:
                 [0, 1], first and last the pairs that make "beta_fast" (32) and "beta_slow"
                 (1) turns r over "original_max_position" rows L,
                 rotary_dim ln(L / (2 pi r)) / (2 ln theta), rounded down and up (not with
-                "truncate" false): what a config.json means; and the rotated columns times "attention_factor"
-                (default 0.1 ln s + 1).  "ramp": "turns" instead of "pairs": a line in
-                the turns, g = (beta_fast - r) / (beta_fast - beta_slow)
+                "truncate" false): what a config.json means; and the rotated columns
+                times "attention_factor" (default 0.1 ln s + 1).  "ramp": "turns" instead
+                of "pairs": a line in the turns, g = (beta_fast - r) / (beta_fast - beta_slow)
     frequencies: a sequence of rotary_dim / 2 numbers instead of all that."""
 
     def __init__(self, rotary_dim: int = 64, theta: float = 1e7, layout: str = "half",
